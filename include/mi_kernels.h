@@ -412,6 +412,154 @@ int mi_top_p_sample_batched_f16(const void* logits, int64_t B, int64_t vocab, fl
  * mirror only.  Returns the previous mode, or MI_ERR_INVALID_ARGUMENT. */
 int mi_exchange_test_mode(int mode);
 
+/* ---- rotary positions in other layouts ------------------------------------ */
+
+/* Rotary positions over the first rotary_dim elements of each head, in either
+ * layout, from or into rows that may be slices of a fused QKV product (no
+ * counterpart in the reference, whose RoPE is mi_rope_neox_qk_f16's):
+ *   (c, s) = mscale * (cos, sin)(positions[t] * inv_freq_host[i]),
+ *   y1 = x1 c - x2 s,  y2 = x2 c + x1 s,  i < rotary_dim / 2,
+ * with (x1, x2) = x[i], x[i + rotary_dim/2], or x[2i], x[2i+1] when
+ * interleaved.  The angle is the exact product (|position| < 2^52), cos and
+ * sin are not rounded to fp16, each output is rounded once; the elements
+ * behind rotary_dim are copied.  q [T, Hq, hd], k [T, Hkv, hd] (NULL when
+ * Hkv == 0) with tokens q_stride / k_stride elements apart (>= Hq * hd,
+ * Hkv * hd; any value when T <= 1), likewise q_out, k_out: the inputs
+ * themselves with their strides (in place: only the rotated part is read and
+ * written), or rows that no input row and no other output row shares a byte
+ * with (else MI_ERR_ALIASING).  inv_freq_host: rotary_dim/2 finite HOST floats,
+ * passed by value.  rotary_dim even, <= 512; interleaved pairs 4-byte aligned
+ * (else MI_ERR_UNSUPPORTED). */
+int mi_rope_partial_qk_f16(const void* q, const void* k, void* q_out, void* k_out,
+                           const int64_t* positions, const float* inv_freq_host, int64_t T,
+                           int64_t Hq, int64_t Hkv, int64_t head_dim, int64_t rotary_dim,
+                           int64_t q_stride, int64_t k_stride, int64_t q_out_stride,
+                           int64_t k_out_stride, int interleaved, float mscale, void* stream);
+
+/* ---- the paged KV cache held in 8 bits ------------------------------------- */
+
+/* A cache is k_cache / v_cache [L, num_blocks, Hkv, block_size, hd] of e4m3
+ * bytes (OCP, no infinities) and k_scale / v_scale [L, num_blocks, Hkv] of one
+ * exponent byte b per page and head (OCP e8m0; 255 is NaN): an element stands
+ * for half(e4m3 * 2^(b - 127)).  (The reference's cache is fp16 only,
+ * src/kernels/model_utils_kernel.cuh:53-67.) */
+
+/* K and V rows [T, Hkv, hd] fp16 (tokens k_stride / v_stride elements apart)
+ * into layer `layer` of an 8-bit cache, by segments (at most 8, over disjoint
+ * token ranges), with the placement and skip rules of
+ * mi_paged_kv_scatter_f16.  Per page and head, e is the least integer in
+ * [-32, 8] with |x| <= 448 * 2^e for the finite values that the call writes
+ * there; if the call writes the page's slot 0, the page begins anew with e,
+ * otherwise it takes max(e, its own), and where that raises its own, its other
+ * slots are rounded again.  Values are rounded to nearest even, held to 61440,
+ * infinities and NaN become NaN; slots behind the written ones hold anything.
+ * A page written by two sequences of a call holds what no order defines.
+ * hd <= 512, block_size <= 4096, Hkv <= 1024, otherwise MI_ERR_UNSUPPORTED. */
+int mi_kv8_scatter_f16(const void* k, const void* v, int64_t k_stride, int64_t v_stride,
+                       int64_t T, int64_t Hkv, int64_t head_dim, void* k_cache, void* v_cache,
+                       void* k_scale, void* v_scale, int64_t layer, int64_t num_blocks,
+                       int64_t block_size, const mi_kv_segment* segments, int num_segments,
+                       void* stream);
+
+/* Causal attention of q [T, Hq, hd] fp16 over layer `layer` of an 8-bit cache,
+ * Hq a multiple of Hkv (query head h reads KV head h / (Hq / Hkv)), by
+ * segments (at most 8, over disjoint token ranges): token (b, s) is at
+ * position p = start_pos[b] + s and sees the sequence's keys 0 .. p, or with
+ * window > 0 the last `window` of them:
+ *   out[t, h] = sum_j softmax_j(scale * q[t, h] . k_j) v_j.
+ * Its own key and value have to be in the cache.  A token at p < 0 or
+ * p >= seq_len[b], or that sees no key, gets zeros; rows in no segment stay as
+ * they were.  Keys whose block lies outside the table or the cache are left
+ * out.  What no token sees may hold anything, NaN included.  Sums are fp32,
+ * the softmax's weights are rounded to fp16.  The cached values have to be
+ * within fp16's range, as mi_kv8_scatter_f16 leaves them.
+ * hd a multiple of 16 (<= 256), block_size a multiple of 16 (<= 4096), at most
+ * 2^25 keys per sequence, q and the caches 16-byte aligned and q_stride a
+ * multiple of 8; otherwise MI_ERR_UNSUPPORTED.  out must not overlap
+ * anything.  The workspace (mi_kv8_attention_workspace_bytes(Hq, Hkv, hd,
+ * segments) bytes, 16-byte aligned, may be NULL when that is 0; by the
+ * segments' B, S and max_blocks_per_seq alone) must hold zeros before its
+ * first use and then serve only this function; calls sharing it must not
+ * overlap in time. */
+int64_t mi_kv8_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t head_dim,
+                                         const mi_kv_segment* segments, int num_segments);
+int mi_kv8_attention_f16(const void* q, int64_t q_stride, const void* k_cache,
+                         const void* v_cache, const void* k_scale, const void* v_scale, void* out,
+                         int64_t out_stride, int64_t T, int64_t Hq, int64_t Hkv,
+                         int64_t head_dim, float scale, int64_t window, int64_t layer,
+                         int64_t num_blocks, int64_t block_size, const mi_kv_segment* segments,
+                         int num_segments, void* workspace, int64_t workspace_bytes,
+                         void* stream);
+
+/* ---- the pages of a cache ---------------------------------------------------- */
+
+/* One tensor [layers, num_blocks, page_bytes] of a paged cache: K or V of
+ * either type, or their scales.  A call takes at most 8. */
+typedef struct mi_kv_pages {
+    void* data;
+    int64_t layers;
+    int64_t page_bytes;
+} mi_kv_pages;
+
+/* What became of a listed row or pair (int32 DEVICE status arrays). */
+#define MI_KV_DONE 0
+#define MI_KV_FULL 1    /* no pages left for it: nothing was changed */
+#define MI_KV_REFUSED 2 /* not a row or page, or one that the call may not touch */
+
+/* The calls below keep a cache's pages on the device: block_table [B,
+ * max_blocks_per_seq] (-1: no page), seq_len [B], and ref_count [num_blocks],
+ * the number of table entries that hold a page (0: free).  All arrays are
+ * int32 DEVICE arrays; status, moved and the workspace overlap nothing else.
+ * What a call leaves depends on the state and the call alone: free pages are
+ * taken lowest first, rows are served in the order listed. */
+
+/* Pages src[i] -> dst[i] in every cache and layer, i < n (<= 2^20).  A pair is
+ * refused, and copies nothing, when a page of it lies outside the cache or its
+ * dst is another pair's src or an earlier pair's dst (so a pair may be served
+ * whose source another pair shares). */
+int mi_kv_pages_copy(const mi_kv_pages* caches, int num_caches, int64_t num_blocks,
+                     const int* src, const int* dst, int64_t n, int* status, void* stream);
+
+/* Rows rows[i], i < n (<= 2^20), give up their pages and become empty (length
+ * 0, entries -1); a page with no other holder is free.  Rows outside the table
+ * are passed over, and so is a row's second listing. */
+int mi_kv_pages_free(int* block_table, int* seq_len, int* ref_count, int64_t B,
+                     int64_t max_blocks_per_seq, int64_t num_blocks, const int* rows, int64_t n,
+                     void* stream);
+
+/* Row children[i], which has to be empty, becomes a second holder of all pages
+ * of row parents[i], at its length, i < n (<= 2^20); a parent may be listed
+ * often.  Refused: rows outside the table, a child that is not empty or listed
+ * before, a parent that is a child of the call.  The last page stays shared
+ * until mi_kv_pages_reserve makes room in it. */
+int mi_kv_pages_fork(int* block_table, int* seq_len, int* ref_count, int64_t B,
+                     int64_t max_blocks_per_seq, int64_t num_blocks, const int* parents,
+                     const int* children, int64_t n, int* status, void* stream);
+
+/* Row rows[i] grows to lengths[i] tokens (a shorter length changes nothing),
+ * i < n (<= 1024): new pages for the blocks that it has none for, and where
+ * its last page is partly full and shared, a copy of that page in all caches
+ * (the last of the holders that are left keeps it), so that the row may then
+ * write behind its old end.  Rows are served in order; the first that the free
+ * pages do not reach for, and all behind it, get MI_KV_FULL.  Refused: rows
+ * outside the table or listed before, lengths beyond max_blocks_per_seq *
+ * block_size (< 2^31).  Workspace: mi_kv_pages_workspace_bytes(num_blocks, n)
+ * bytes of any content. */
+int64_t mi_kv_pages_workspace_bytes(int64_t num_blocks, int64_t n);
+int mi_kv_pages_reserve(const mi_kv_pages* caches, int num_caches, int* block_table, int* seq_len,
+                        int* ref_count, int64_t B, int64_t max_blocks_per_seq, int64_t num_blocks,
+                        int64_t block_size, const int* rows, const int* lengths, int64_t n,
+                        int* status, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* Moves the live pages to the front: with n of them, the live pages at or
+ * behind n, in order, take the free pages before n, in all caches, in
+ * ref_count and in the table.  moved [num_blocks] gets each page's new place,
+ * -1 for a page that was free.  Workspace: mi_kv_pages_workspace_bytes(
+ * num_blocks, 0) bytes of any content. */
+int mi_kv_pages_compact(const mi_kv_pages* caches, int num_caches, int* block_table,
+                        int* ref_count, int64_t B, int64_t max_blocks_per_seq, int64_t num_blocks,
+                        int* moved, void* workspace, int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

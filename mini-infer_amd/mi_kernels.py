@@ -74,6 +74,20 @@ SIGNATURES = {
     "mi_greedy_argmax_test_poll_limit": [_int],
     "mi_exchange_test_mode": [_int],
     "mi_abi_version": [],
+    "mi_rope_partial_qk_f16": [_c_void_p] * 6 + [_i64] * 9 + [_int, _f32, _c_void_p],
+    "mi_kv8_scatter_f16": [_c_void_p] * 2 + [_i64] * 5 + [_c_void_p] * 4 + [_i64] * 3
+                          + [_c_void_p, _int, _c_void_p],
+    "mi_kv8_attention_workspace_bytes": [_i64] * 3 + [_c_void_p, _int],
+    "mi_kv8_attention_f16": [_c_void_p, _i64] + [_c_void_p] * 5 + [_i64] * 5 + [_f32] + [_i64] * 4
+                            + [_c_void_p, _int, _c_void_p, _i64, _c_void_p],
+    "mi_kv_pages_copy": [_c_void_p, _int, _i64, _c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p],
+    "mi_kv_pages_free": [_c_void_p] * 3 + [_i64] * 3 + [_c_void_p, _i64, _c_void_p],
+    "mi_kv_pages_fork": [_c_void_p] * 3 + [_i64] * 3 + [_c_void_p] * 2 + [_i64] + [_c_void_p] * 2,
+    "mi_kv_pages_workspace_bytes": [_i64, _i64],
+    "mi_kv_pages_reserve": [_c_void_p, _int] + [_c_void_p] * 3 + [_i64] * 4 + [_c_void_p] * 2
+                           + [_i64, _c_void_p, _c_void_p, _i64, _c_void_p],
+    "mi_kv_pages_compact": [_c_void_p, _int] + [_c_void_p] * 2 + [_i64] * 3
+                           + [_c_void_p, _c_void_p, _i64, _c_void_p],
 }
 
 _lib = None
@@ -99,6 +113,8 @@ def load_library(path: os.PathLike | str | None = None) -> ctypes.CDLL:
     lib.mi_softmax_workspace_bytes.restype = _i64
     lib.mi_softmax_argmax_workspace_bytes.argtypes = [_i64, _i64]
     lib.mi_softmax_argmax_workspace_bytes.restype = _i64
+    lib.mi_kv8_attention_workspace_bytes.restype = _i64
+    lib.mi_kv_pages_workspace_bytes.restype = _i64
     lib.mi_status_string.argtypes = [_int]
     lib.mi_status_string.restype = ctypes.c_char_p
     if path is None:
@@ -881,3 +897,381 @@ def greedy_argmax(logits, out=None, workspace=None, stream=None):
         _check(lib.mi_greedy_argmax_ws_f16(_ptr(x), B, V, _ptr(out), _ptr(workspace), nbytes,
                                            _stream(stream)), "mi_greedy_argmax_ws_f16")
     return out
+
+
+# ---------------------------------------------------------------------------
+# Rotary positions in other layouts
+# ---------------------------------------------------------------------------
+
+def rope_scaled_inv_freq(rotary_dim: int, theta: float = 1e6, scaling: str = "none",
+                         factor: float = 1.0, original_len: int = 4096, low: float = 1.0,
+                         high: float = 32.0):
+    """(inv_freq float32 [rotary_dim / 2], mscale) for rope_partial_qk, with the
+    frequencies f_i = theta^(-2i / rotary_dim) scaled for contexts `factor` times
+    as long as the original_len tokens that the model was trained on:
+
+    "none"    as they are
+    "linear"  f_i / factor: positions interpolated
+    "ntk"     theta * factor^(r / (r - 2)): the lowest frequency is divided by
+              factor, the highest kept
+    "bands"   f_i that turn fewer than `low` times over original_len are divided by
+              factor, those that turn more than `high` times are kept, and between
+              them both forms are mixed, linearly in the turns
+    "yarn"    as "bands", mixed linearly in the dimension's index (Peng et al.,
+              "YaRN", 2023), with mscale = 0.1 ln(factor) + 1
+    """
+    import math  # noqa: PLC0415
+    import numpy as np  # noqa: PLC0415
+    r = int(rotary_dim)
+    if r <= 0 or r % 2:
+        raise ValueError("rotary_dim must be even and positive")
+    if not (factor >= 1.0 and theta > 1.0 and original_len > 0 and 0 < low < high):
+        raise ValueError("need factor >= 1, theta > 1, original_len > 0 and 0 < low < high")
+    i = np.arange(0, r, 2, dtype=np.float64) / r
+    f = theta ** -i
+    mscale = 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "ntk":
+        if r > 2:
+            f = (theta * factor ** (r / (r - 2))) ** -i
+    elif scaling == "bands":
+        keep = np.clip((original_len * f / (2 * math.pi) - low) / (high - low), 0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+    elif scaling == "yarn":
+        def index(turns):  # of the dimension that turns so often
+            return r * math.log(original_len / (turns * 2 * math.pi)) / (2 * math.log(theta))
+        a, b = max(math.floor(index(high)), 0), min(math.ceil(index(low)), r - 1)
+        keep = 1.0 - np.clip((np.arange(r // 2) - a) / max(b - a, 1e-3), 0.0, 1.0)
+        f = f * keep + f / factor * (1.0 - keep)
+        mscale = 0.1 * math.log(factor) + 1.0
+    elif scaling != "none":
+        raise ValueError(f"unknown scaling {scaling!r}")
+    return f.astype(np.float32), mscale
+
+
+def _current(t, name: str) -> None:
+    """A call goes to a stream of the current device: so must its tensors."""
+    if t.device.index != _torch().cuda.current_device():
+        raise ValueError(f"{name} is on {t.device}, not on the current device "
+                         f"(cuda:{_torch().cuda.current_device()})")
+
+
+def _need_rows(t, name: str):
+    """A [T, H, hd] fp16 GPU tensor whose tokens are contiguous rows, any distance
+    apart (a slice of a fused product's rows); returns that distance."""
+    torch = _torch()
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.device.type != "cuda":
+        raise ValueError(f"{name} must be on the GPU, got {t.device}")
+    if t.dtype != torch.float16:
+        raise TypeError(f"{name} must be {torch.float16}, got {t.dtype}")
+    if t.dim() != 3:
+        raise ValueError(f"{name} must be 3-D [T, H, head_dim]")
+    _current(t, name)
+    T, H, hd = t.shape
+    if t.numel() == 0 or (T == 1 and t.is_contiguous()):
+        return H * hd
+    s = t.stride()
+    if (hd > 1 and s[2] != 1) or (H > 1 and s[1] != hd) or (T > 1 and s[0] < H * hd):
+        raise ValueError(f"{name}: each token's [H, head_dim] must be contiguous, got strides {s}")
+    return s[0] if T > 1 else H * hd
+
+
+def rope_partial_qk(q, k, positions, inv_freq, interleaved: bool = False, mscale: float = 1.0,
+                    q_out=None, k_out=None, stream=None):
+    """Rotary positions of q [T, Hq, hd] and k [T, Hkv, hd] (k may be None) over the
+    first 2 * len(inv_freq) elements of each head, as halves or as interleaved
+    pairs, cos and sin times mscale; tokens may be any distance apart (slices of
+    a fused QKV product).  In place, or into q_out / k_out.  Returns (q_out, k_out)."""
+    torch = _torch()
+    qs = _need_rows(q, "q")
+    T, Hq, hd = q.shape
+    _need(positions, torch.int64, "positions")
+    _current(positions, "positions")
+    if positions.numel() != T:
+        raise ValueError("positions must hold T entries")
+    ks = Hkv = 0
+    if k is not None:
+        ks = _need_rows(k, "k")
+        if k.shape[0] != T or k.shape[2] != hd:
+            raise ValueError("k must be [T, Hkv, hd]")
+        Hkv = k.shape[1]
+    elif k_out is not None:
+        raise ValueError("k_out without k")
+    q_out = q if q_out is None else q_out
+    k_out = k if k_out is None else k_out
+    qos, kos = _need_rows(q_out, "q_out"), _need_rows(k_out, "k_out") if k is not None else 0
+    if q_out.shape != q.shape or (k is not None and k_out.shape != k.shape):
+        raise ValueError("q_out / k_out must have the inputs' shapes")
+    arr, p = _inv_freq_buffer(inv_freq)
+    if arr.ndim != 1 or arr.size == 0 or 2 * arr.size > hd:
+        raise ValueError("inv_freq must hold up to head_dim/2 entries")
+    null = ctypes.c_void_p(0)
+    _check(load_library().mi_rope_partial_qk_f16(
+        _ptr(q), _ptr(k) if k is not None else null, _ptr(q_out),
+        _ptr(k_out) if k is not None else null, _ptr(positions), p, T, Hq, Hkv, hd, 2 * arr.size,
+        qs, ks, qos, kos, int(bool(interleaved)), float(mscale), _stream(stream)),
+        "mi_rope_partial_qk_f16")
+    return q_out, k_out
+
+
+# ---------------------------------------------------------------------------
+# The paged KV cache held in 8 bits
+# ---------------------------------------------------------------------------
+
+def kv8_cache(num_layers: int, num_blocks: int, num_kv_heads: int, block_size: int, head_dim: int,
+              device="cuda"):
+    """(k_cache, v_cache, k_scale, v_scale) of an empty 8-bit cache: e4m3 [L, num_blocks,
+    Hkv, block_size, hd], and one exponent byte per page and head, uint8 [L,
+    num_blocks, Hkv]; an element stands for e4m3 * 2^(byte - 127)."""
+    torch = _torch()
+    shape = (num_layers, num_blocks, num_kv_heads, block_size, head_dim)
+    k, v = (torch.zeros(shape, dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+            for _ in range(2))
+    ks, vs = (torch.full(shape[:3], 127, dtype=torch.uint8, device=device) for _ in range(2))
+    return k, v, ks, vs
+
+
+def _kv8_checks(k_cache, v_cache, k_scale, v_scale, layer, on):
+    torch = _torch()
+    for t, n in ((k_cache, "k_cache"), (v_cache, "v_cache")):
+        _need(t, torch.float8_e4m3fn, n)
+    for t, n in ((k_scale, "k_scale"), (v_scale, "v_scale")):
+        _need(t, torch.uint8, n)
+    if k_cache.dim() != 5 or v_cache.shape != k_cache.shape:
+        raise ValueError("caches must be [L, num_blocks, Hkv, bs, hd], equal shapes")
+    if k_scale.shape != k_cache.shape[:3] or v_scale.shape != k_cache.shape[:3]:
+        raise ValueError("scales must be [L, num_blocks, Hkv]")
+    if not 0 <= layer < k_cache.shape[0]:
+        raise ValueError("layer lies outside the cache")
+    for t in (k_cache, v_cache, k_scale, v_scale):
+        if t.device != on.device:
+            raise ValueError(f"all tensors must be on {on.device}, got {t.device}")
+    return k_cache.shape
+
+
+def _kv8_segments(segments):
+    for g in segments:
+        for n in ("block_table", "seq_len", "start_pos"):
+            if isinstance(g[n], _torch().Tensor) and g[n].device.type == "cuda":
+                _current(g[n], n)
+    return _kv_segments(segments)
+
+
+def kv8_scatter(k, v, k_cache, v_cache, k_scale, v_scale, layer: int, segments, stream=None):
+    """Writes k, v [T, Hkv, hd] (tokens any distance apart) into layer `layer` of an 8-bit cache
+    (kv8_cache) for the tokens of `segments` (as rope_kv_scatter's): each page and head
+    takes the least power-of-two scale that holds its largest value; see
+    mi_kv8_scatter_f16."""
+    L, NB, Hkv, bs, hd = _kv8_checks(k_cache, v_cache, k_scale, v_scale, layer, k)
+    ks, vs = _need_rows(k, "k"), _need_rows(v, "v")
+    T = k.shape[0]
+    if tuple(k.shape) != (T, Hkv, hd) or v.shape != k.shape:
+        raise ValueError("k and v must be [T, Hkv, hd] as the cache is")
+    segs = _kv8_segments(segments)
+    _check(load_library().mi_kv8_scatter_f16(
+        _ptr(k), _ptr(v), ks, vs, T, Hkv, hd, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale),
+        _ptr(v_scale), layer, NB, bs, segs, len(segments), _stream(stream)), "mi_kv8_scatter_f16")
+    return k_cache, v_cache
+
+
+def kv8_attention_workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: int, segments) -> int:
+    segs = _kv8_segments(segments)
+    n = int(load_library().mi_kv8_attention_workspace_bytes(num_heads, num_kv_heads, head_dim,
+                                                            segs, len(segments)))
+    if n < 0:
+        _check(n, "mi_kv8_attention_workspace_bytes")
+    return n
+
+
+def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, layer: int, segments, scale=None,
+                  window: int = 0, out=None, workspace=None, stream=None):
+    """Causal attention of q [T, Hq, hd] (tokens any distance apart) over layer `layer` of an 8-bit
+    cache for the tokens of `segments` (as rope_kv_scatter's; the tokens' own K and V are
+    in the cache): softmax(scale * q . k) v over each token's position and those before
+    it, or the last `window` of them; scale: 1 / sqrt(hd) if None.  A new `out` is
+    zeros where no segment has the token.  `workspace`
+    (kv8_attention_workspace_bytes) must be zero before its first use and kept for
+    this function; without one, a call makes its own.  Returns out."""
+    torch = _torch()
+    qs = _need_rows(q, "q")
+    T, Hq, hd = q.shape
+    L, NB, Hkv, bs, Dc = _kv8_checks(k_cache, v_cache, k_scale, v_scale, layer, q)
+    if Dc != hd or Hkv == 0 or Hq % Hkv:
+        raise ValueError("q must be [T, Hq, hd] with the cache's hd and a multiple of its heads")
+    if scale is None:
+        scale = hd ** -0.5
+    segs = _kv8_segments(segments)
+    if out is None:
+        out = torch.zeros((T, Hq, hd), dtype=torch.float16, device=q.device)
+    os_ = _need_rows(out, "out")
+    if out.shape != q.shape or out.device != q.device:
+        raise ValueError("out must have q's shape and device")
+    if workspace is None:
+        n = kv8_attention_workspace_bytes(Hq, Hkv, hd, segments)
+        workspace = torch.zeros(max(n, 16), dtype=torch.uint8, device=q.device)
+        if stream is not None:
+            workspace.record_stream(stream)
+    elif workspace.device != q.device or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous tensor on q's device")
+    _check(load_library().mi_kv8_attention_f16(
+        _ptr(q), qs, _ptr(k_cache), _ptr(v_cache), _ptr(k_scale), _ptr(v_scale), _ptr(out), os_, T,
+        Hq, Hkv, hd, float(scale), int(window), layer, NB, bs, segs, len(segments),
+        _ptr(workspace), workspace.numel() * workspace.element_size(), _stream(stream)),
+        "mi_kv8_attention_f16")
+    return out
+
+
+# ---------------------------------------------------------------------------
+# The pages of a cache
+# ---------------------------------------------------------------------------
+
+KV_DONE, KV_FULL, KV_REFUSED = 0, 1, 2
+
+
+class KvPages(ctypes.Structure):
+    """mi_kv_pages: one tensor [layers, num_blocks, page_bytes] of a cache."""
+    _fields_ = [("data", _c_void_p), ("layers", _i64), ("page_bytes", _i64)]
+
+
+def _page_caches(caches, num_blocks, on):
+    torch = _torch()
+    arr = (KvPages * max(1, len(caches)))()
+    for i, c in enumerate(caches):
+        if not isinstance(c, torch.Tensor):
+            raise TypeError(f"caches[{i}] must be a torch.Tensor")
+        if c.device != on.device or not c.is_contiguous():
+            raise ValueError(f"caches[{i}] must be contiguous, on {on.device}")
+        if c.dim() < 2 or (num_blocks is not None and c.shape[1] != num_blocks) or \
+                c.shape[1] != caches[0].shape[1]:
+            raise ValueError("caches must be [L, num_blocks, ...], with one number of blocks (num_blocks)")
+        arr[i].data = _ptr(c).value
+        arr[i].layers = c.shape[0]
+        arr[i].page_bytes = c[0, 0].numel() * c.element_size() if c.numel() else 0
+    return arr
+
+
+def _page_ints(on, *named):
+    torch = _torch()
+    for t, n in named:
+        _need(t, torch.int32, n)
+        if t.device != on.device:
+            raise ValueError(f"{n} must be on {on.device}, got {t.device}")
+
+
+def _page_state(block_table, seq_len, ref_count):
+    _page_ints(block_table, (block_table, "block_table"), (ref_count, "ref_count"))
+    _current(block_table, "block_table")
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [B, max_blocks]")
+    B, mb = block_table.shape
+    if seq_len is not None:
+        _page_ints(block_table, (seq_len, "seq_len"))
+        if seq_len.numel() != B:
+            raise ValueError("seq_len must hold B entries")
+    return B, mb, ref_count.numel()
+
+
+def _status(status, n, on):
+    torch = _torch()
+    if status is None:
+        return torch.empty(n, dtype=torch.int32, device=on.device)
+    _page_ints(on, (status, "status"))
+    if status.numel() != n:
+        raise ValueError(f"status must hold {n} entries")
+    return status
+
+
+def _page_workspace(workspace, num_blocks, n, on, stream):
+    torch = _torch()
+    need = int(load_library().mi_kv_pages_workspace_bytes(num_blocks, n))
+    if workspace is None:
+        workspace = torch.empty(need // 4, dtype=torch.int32, device=on.device)
+        if stream is not None:
+            workspace.record_stream(stream)
+    elif workspace.device != on.device or not workspace.is_contiguous():
+        raise ValueError("workspace must be a contiguous tensor on the cache's device")
+    return workspace, workspace.numel() * workspace.element_size()
+
+
+def kv_pages_workspace_bytes(num_blocks: int, n: int) -> int:
+    return int(load_library().mi_kv_pages_workspace_bytes(num_blocks, n))
+
+
+def kv_copy_pages(caches, src, dst, status=None, stream=None):
+    """Copies pages src[i] -> dst[i] (int32, on the GPU) in every tensor of `caches` ([L,
+    num_blocks, ...], any type) and layer.  Returns status [n]: KV_DONE, or KV_REFUSED
+    for a pair whose pages lie outside or whose dst is another pair's src or an
+    earlier pair's dst."""
+    if not caches:
+        raise ValueError("caches must hold at least one tensor")
+    _page_ints(src, (src, "src"), (dst, "dst"))
+    _current(src, "src")
+    n = src.numel()
+    if dst.numel() != n:
+        raise ValueError("src and dst must have as many entries")
+    arr = _page_caches(caches, None, src)
+    status = _status(status, n, src)
+    _check(load_library().mi_kv_pages_copy(arr, len(caches), caches[0].shape[1], _ptr(src),
+                                           _ptr(dst), n, _ptr(status), _stream(stream)),
+           "mi_kv_pages_copy")
+    return status
+
+
+def kv_free(block_table, seq_len, ref_count, rows, stream=None):
+    """Rows `rows` (int32) of block_table [B, max_blocks] give up their pages and become empty."""
+    B, mb, NB = _page_state(block_table, seq_len, ref_count)
+    _page_ints(block_table, (rows, "rows"))
+    _check(load_library().mi_kv_pages_free(_ptr(block_table), _ptr(seq_len), _ptr(ref_count), B, mb,
+                                           NB, _ptr(rows), rows.numel(), _stream(stream)),
+           "mi_kv_pages_free")
+
+
+def kv_fork(block_table, seq_len, ref_count, parents, children, status=None, stream=None):
+    """Row children[i], which has to be empty, comes to share all pages of row parents[i].  Returns
+    status [n] (KV_DONE or KV_REFUSED)."""
+    B, mb, NB = _page_state(block_table, seq_len, ref_count)
+    _page_ints(block_table, (parents, "parents"), (children, "children"))
+    n = parents.numel()
+    if children.numel() != n:
+        raise ValueError("parents and children must have as many entries")
+    status = _status(status, n, block_table)
+    _check(load_library().mi_kv_pages_fork(_ptr(block_table), _ptr(seq_len), _ptr(ref_count), B, mb,
+                                           NB, _ptr(parents), _ptr(children), n, _ptr(status),
+                                           _stream(stream)), "mi_kv_pages_fork")
+    return status
+
+
+def kv_reserve(caches, block_table, seq_len, ref_count, rows, lengths, block_size: int,
+               status=None, workspace=None, stream=None):
+    """Row rows[i] grows to lengths[i] tokens: new pages, and a copy of its last page in all caches
+    where that is partly full and shared.  Returns status [n] (KV_DONE, KV_FULL where
+    the free pages did not reach, KV_REFUSED)."""
+    B, mb, NB = _page_state(block_table, seq_len, ref_count)
+    _page_ints(block_table, (rows, "rows"), (lengths, "lengths"))
+    n = rows.numel()
+    if lengths.numel() != n:
+        raise ValueError("rows and lengths must have as many entries")
+    arr = _page_caches(caches, NB, block_table)
+    status = _status(status, n, block_table)
+    ws, nbytes = _page_workspace(workspace, NB, n, block_table, stream)
+    _check(load_library().mi_kv_pages_reserve(arr, len(caches), _ptr(block_table), _ptr(seq_len),
+                                              _ptr(ref_count), B, mb, NB, block_size, _ptr(rows),
+                                              _ptr(lengths), n, _ptr(status), _ptr(ws), nbytes,
+                                              _stream(stream)), "mi_kv_pages_reserve")
+    return status
+
+
+def kv_compact(caches, block_table, ref_count, moved=None, workspace=None, stream=None):
+    """Moves the live pages to the front of the cache, in all caches, in ref_count and in the
+    table.  Returns moved [num_blocks]: each page's new place, -1 for one that was free."""
+    B, mb, NB = _page_state(block_table, None, ref_count)
+    arr = _page_caches(caches, NB, block_table)
+    moved = _status(moved, NB, block_table)
+    ws, nbytes = _page_workspace(workspace, NB, 0, block_table, stream)
+    _check(load_library().mi_kv_pages_compact(arr, len(caches), _ptr(block_table), _ptr(ref_count),
+                                              B, mb, NB, _ptr(moved), _ptr(ws), nbytes,
+                                              _stream(stream)), "mi_kv_pages_compact")
+    return moved
