@@ -29,7 +29,9 @@ constexpr int kRows = 16;      // query rows of a tile: (token, head of the KV h
 constexpr int kKeys = 64;      // keys of a wave's step
 constexpr int kWaves = 4;      // waves of a workgroup, each on every fourth step
 constexpr float kPShift = 14.0f;
-constexpr int64_t kMaxSplits = 128;
+constexpr int kMaxSplits = 64;
+constexpr int64_t kWant = 2048;                  // workgroups that a segment is split into at most
+constexpr int64_t kCounters = kKv8Segs * kWant;  // at the head of the workspace, zeros between calls
 
 struct Kv8Attn {
     const half_t* q;
@@ -39,6 +41,8 @@ struct Kv8Attn {
     int Hq, Hkv, G, hd, bs, window;
     float c;  // scale * log2(e)
     float* part;  // [slot][row][hd + 2]: sums, then maximum and sum of weights
+    unsigned* count;  // splits done, per (sequence, tile, KV head) of the segments in splits
+    int64_t unsplit[kKv8Segs];  // such groups of the segments before that are in none
     Kv8Segs sg;
     int tiles[kKv8Segs], nsplit[kKv8Segs];
     int64_t first[kKv8Segs + 1];  // a segment's first workgroup, and its first slot
@@ -68,12 +72,19 @@ __device__ __forceinline__ TileKeys tile_keys(const Kv8Attn& a, int g, int64_t b
     t.lo = a.window > 0 ? max<int64_t>(first - a.window + 1, 0) : 0;
     if (last < first) t.hi = t.lo = 0;
     t.base = t.lo & ~int64_t{15};
-    t.steps = t.hi > t.lo ? static_cast<int>((t.hi - t.base + kKeys - 1) / kKeys) : 0;
+    t.steps = t.hi > t.lo && a.num_blocks > 0 ? static_cast<int>((t.hi - t.base + kKeys - 1) / kKeys) : 0;
     const int ns = a.nsplit[g];
     t.per = max((t.steps + ns - 1) / ns, kWaves);
     t.per = (t.per + kWaves - 1) / kWaves * kWaves;
     t.used = (t.steps + t.per - 1) / t.per;
     return t;
+}
+
+// id % d; id becomes id / d.
+__device__ __forceinline__ int divmod(uint32_t& id, int d) {
+    const uint32_t q = id / static_cast<uint32_t>(d), r = id - q * static_cast<uint32_t>(d);
+    id = q;
+    return static_cast<int>(r);
 }
 
 __device__ __forceinline__ float max_over_groups(float v) {
@@ -88,12 +99,23 @@ __device__ __forceinline__ float sum_over_groups(float v) {
     return v + __shfl_xor(v, 32, kWave);
 }
 
-// Loads of W dwords where `ok`, zeros elsewhere.
+// What a partial sum with maximum m and sum of weights l counts, beside the maximum ref;
+// one that saw nothing counts nothing, and one of NaN alone (m stays -inf) must not be lost.
+__device__ __forceinline__ float join_weight(float m, float l, float ref) {
+    return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m - ref);
+}
+
+__device__ __forceinline__ void store_agent(float* p, float v) {
+    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float load_agent(const float* p) {
+    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+
 template <int W>
-__device__ __forceinline__ void load_words(uint32_t* to, const uint8_t* p, bool ok) {
+__device__ __forceinline__ void load_words(uint32_t* to, const uint8_t* p) {
     typedef uint32_t vec __attribute__((ext_vector_type(W)));
-    vec v = vec(0);
-    if (ok) v = *reinterpret_cast<const vec*>(p);
+    const vec v = *reinterpret_cast<const vec*>(p);
 #pragma unroll
     for (int i = 0; i < W; ++i) to[i] = v[i];
 }
@@ -131,14 +153,10 @@ __device__ __forceinline__ void v_pair(const uint32_t (&raw)[16][Tile<HD>::kVw],
     odd = __builtin_bit_cast(h8, u4{o[0], o[1], o[2], o[3]});
 }
 
-// NaN elements of v to 0, and ones in their places in `nan`.
-__device__ __forceinline__ void split_nan(h8& v, h8& nan) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const bool is = v[i] != v[i];
-        nan[i] = is ? (half_t)1.0f : (half_t)0.0f;
-        if (is) v[i] = (half_t)0.0f;
-    }
+// All bits of the bytes of w that are NaN.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+    const uint32_t top = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+    return top | (top - (top >> 7));
 }
 
 // One workgroup: a tile of 16 rows of one sequence and KV head, over one split of its keys.
@@ -147,22 +165,21 @@ __device__ __forceinline__ void split_nan(h8& v, h8& nan) {
 // read once the scores are made, V of the next after the sums, so a wave always has half a
 // step (8 KB at head_dim 128) in flight while it computes.
 template <int HD>
-__global__ __launch_bounds__(256, 2) void kv8_attn_kernel(Kv8Attn a) {
+__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn a) {
     using L = Tile<HD>;
     __shared__ float s_ml[kWaves][2][kRows];
     __shared__ float s_o[kWaves][kRows][HD + 4];
+    __shared__ bool s_last;
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    int64_t id = blockIdx.x;
+    uint32_t id = blockIdx.x;
     int g = 0;
-    while (id >= a.first[g + 1]) ++g;
-    id -= a.first[g];
-    const int h = static_cast<int>(id % a.Hkv);
-    id /= a.Hkv;
-    const int split = static_cast<int>(id % a.nsplit[g]);
-    id /= a.nsplit[g];
-    const int tile = static_cast<int>(id % a.tiles[g]);
-    const int64_t b = id / a.tiles[g];
+    while (id >= static_cast<uint32_t>(a.first[g + 1])) ++g;
+    id -= static_cast<uint32_t>(a.first[g]);
+    const int h = divmod(id, a.Hkv);
+    const int split = divmod(id, a.nsplit[g]);
+    const int tile = divmod(id, a.tiles[g]);
+    const int64_t b = id;
     const TileKeys t = tile_keys(a, g, b, tile);
     if (split >= max(t.used, 1)) return;
     const int col = lane & 15, grp = lane >> 4;
@@ -182,45 +199,49 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(Kv8Attn a) {
         if (live && d < a.hd) qf[i] = ld8(a.q + (tok0 + s) * a.qs + head * a.hd + d);
     }
 
-    // the page of a 16-key block, -1 where it has none
+    // The page of a 16-key block, -1 where it has none.  Every load is unconditional --
+    // of the table's entry 0 or of page 0 where there is none, of the row's first bytes
+    // where head_dim ends before the lane's -- since a load in a branch is waited for there.
     const int* const table = a.sg.bt[g] + b * a.sg.mb[g];
     const int sub = a.bs >> 4;  // 16-key blocks of a page
     const float inv_sub = 1.0f / static_cast<float>(sub);
+    const int nb = static_cast<int>(a.num_blocks);
+    const int end = min((split + 1) * t.per, t.steps);
+    const int base32 = static_cast<int>(t.base);  // <= 2^25
+    const int hi32 = min(static_cast<int>(t.hi), base32 + end * kKeys);
     const auto page_of = [&](int step, int blk, int& in_page) {
-        const int64_t key = t.base + static_cast<int64_t>(step) * kKeys + blk * 16;
-        const int k16 = static_cast<int>(key >> 4);  // < 2^22
+        const int key = base32 + step * kKeys + blk * 16;
+        const int k16 = key >> 4;  // < 2^22
         const int idx = small_div(k16, inv_sub);
         in_page = (k16 - idx * sub) * 16;
-        if (key >= t.hi) return -1;
-        const int phys = table[idx];
-        return phys >= 0 && phys < a.num_blocks ? phys : -1;
+        const int phys = table[key < hi32 ? idx : 0];
+        return key < hi32 && static_cast<uint32_t>(phys) < static_cast<uint32_t>(nb) ? phys : -1;
     };
-    const auto at = [&](int phys) { return (a.layer * a.num_blocks + phys) * a.Hkv + h; };
-
+    const int64_t page0 = a.layer * a.num_blocks;
     uint32_t kr[4][L::kKw], vr[16][L::kVw];
-    float kscale = 1.0f, vscale = 1.0f;
-    const auto load_k = [&](int step) {
-        int in_page;
-        const int phys = page_of(step, col >> 2, in_page);
-        const int64_t pg = at(max(phys, 0));
-        const uint8_t* p = a.kc + (pg * a.bs + in_page + (col & 3)) * a.hd + grp * (HD / 4);
+    int kbyte = 0, vbyte = 0, kphys = -1, vphys = -1, kin = 0, vin = 0, vnext = -1, vnin = 0;
+    const auto find_k = [&](int step) { kphys = page_of(step, col >> 2, kin); };
+    const auto find_v = [&](int step) { vnext = page_of(step, grp, vnin); };
+    const auto load_k = [&] {
+        const int64_t pg = (page0 + max(kphys, 0)) * a.Hkv + h;
+        const uint8_t* const p = a.kc + (pg * a.bs + kin + (col & 3)) * a.hd;
 #pragma unroll
         for (int i = 0; i < 4; ++i)
 #pragma unroll
-            for (int w = 0; w < L::kKw; w += 4)
-                load_words<4>(&kr[i][w], p + i * 4 * a.hd + w * 4, phys >= 0 && grp * (HD / 4) + w * 4 < a.hd);
-        kscale = phys >= 0 ? e8_scale(a.ks[pg]) : 1.0f;
+            for (int w = 0; w < L::kKw; w += 4) {
+                const int d = grp * (HD / 4) + w * 4;
+                load_words<4>(&kr[i][w], p + i * 4 * a.hd + (d < a.hd ? d : 0));
+            }
+        kbyte = a.ks[pg];
     };
-    int vphys = -1;
-    const auto load_v = [&](int step) {
-        int in_page;
-        vphys = page_of(step, grp, in_page);
-        const int64_t pg = at(max(vphys, 0));
-        const uint8_t* p = a.vc + (pg * a.bs + in_page) * a.hd + col * L::kD;
+    const auto load_v = [&] {
+        vphys = vnext;
+        vin = vnin;
+        const int64_t pg = (page0 + max(vphys, 0)) * a.Hkv + h;
+        const uint8_t* const p = a.vc + (pg * a.bs + vin) * a.hd + (col * L::kD < a.hd ? col * L::kD : 0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            load_words<L::kVw>(vr[i], p + i * a.hd, vphys >= 0 && col * L::kD < a.hd);
-        vscale = vphys >= 0 ? e8_scale(a.vs[pg]) : 1.0f;
+        for (int i = 0; i < 16; ++i) load_words<L::kVw>(vr[i], p + i * a.hd);
+        vbyte = a.vs[pg];
     };
 
     f4 o[L::kD];
@@ -231,13 +252,17 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(Kv8Attn a) {
     const int64_t all_hi = min<int64_t>(max<int64_t>(t.sp + t.r0 / a.G, 0) + 1, t.hi);
     const int64_t all_lo = a.window > 0 ? max<int64_t>(t.sp + (t.r0 + t.rows - 1) / a.G - a.window + 1, t.lo) : 0;
     const bool one_pos = t.r0 / a.G == (t.r0 + t.rows - 1) / a.G;
-    const int end = min((split + 1) * t.per, t.steps);
     int step = split * t.per + wave;
     if (step < end) {
-        load_k(step);
-        load_v(step);
+        find_k(step);
+        find_v(step);
+        load_k();
+        load_v();
+        find_k(step + kWaves);
+        find_v(step + kWaves);
     }
     for (; step < end; step += kWaves) {
+        const float kscale = e8_scale(kbyte);
         // scores: tile i's row 4 g + e is key 4 i + e of block g
         f4 sc[4];
 #pragma unroll
@@ -253,11 +278,12 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(Kv8Attn a) {
                 sc[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf, qf[w], sc[i], 0, 0, 0);
             }
         }
-        const int next = step + kWaves;
-        if (next < end) load_k(next);
+        load_k();  // of the next step; behind the last, of whatever page find_k names
+        find_k(step + 2 * kWaves);
+        float vscale = e8_scale(vbyte);
         const int64_t key0 = t.base + static_cast<int64_t>(step) * kKeys;
         const bool masked = key0 + kKeys > all_hi || key0 < all_lo || key0 < t.lo || __any(vphys < 0);
-        uint32_t seen = 0xFFFF;  // of the lane's 16 keys, those that its row sees
+        uint32_t seen_by_any = 0, seen = 0xFFFF;  // of the lane's 16 keys, those that its row sees
         bool nan_path = false;
         float x[16];
 #pragma unroll
@@ -273,16 +299,18 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(Kv8Attn a) {
                 if (!(seen & (1u << i))) x[i] = -INFINITY;
             }
             // what no row sees may hold anything, NaN too: 0 times it must be 0
-            uint32_t nan = vphys >= 0 && (__builtin_bit_cast(uint32_t, vscale) >> 23) == 255 ? some : 0;
+            uint32_t nan = vphys >= 0 && vbyte == 255 ? some : 0;
 #pragma unroll
             for (int i = 0; i < 16; ++i)
 #pragma unroll
                 for (int w = 0; w < L::kVw; ++w) {
                     if (!(some & (1u << i))) vr[i][w] = 0;
-                    nan |= ((vr[i][w] & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+                    nan |= nan_bytes(vr[i][w]);
                 }
             // a NaN that some rows see and others do not
             nan_path = !one_pos && __any(nan != 0);
+            seen_by_any = some;
+            if (vbyte == 255 && (nan_path || some == 0)) vscale = 1.0f;
         }
         float mx = x[0];
 #pragma unroll
@@ -303,33 +331,44 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(Kv8Attn a) {
             l += w;
             p[i >> 3][i & 7] = (half_t)w;
         }
-        if (!nan_path) {
+        if (nan_path) {
 #pragma unroll
-            for (int j = 0; j < L::kD; j += 2)
+            for (int i = 0; i < 16; ++i)
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    h8 even, odd;
-                    v_pair<HD>(vr, k, j >> 2, (j >> 1) & 1, vscale, even, odd);
-                    o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p[k], o[j], 0, 0, 0);
-                    o[j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p[k], o[j + 1], 0, 0, 0);
-                }
-        } else {
+                for (int w = 0; w < L::kVw; ++w) vr[i][w] = vbyte == 255 ? 0u : vr[i][w] & ~nan_bytes(vr[i][w]);
+        }
+#pragma unroll
+        for (int j = 0; j < L::kD; j += 2)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                h8 even, odd;
+                v_pair<HD>(vr, k, j >> 2, (j >> 1) & 1, vscale, even, odd);
+                o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p[k], o[j], 0, 0, 0);
+                o[j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p[k], o[j + 1], 0, 0, 0);
+            }
+        if (nan_path) {  // the rows that see one of the NaN: V again, as ones in their places
+            const int64_t pg = (page0 + max(vphys, 0)) * a.Hkv + h;
+            const uint8_t* const q = a.vc + (pg * a.bs + vin) * a.hd + (col * L::kD < a.hd ? col * L::kD : 0);
             h8 see[2];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) see[i >> 3][i & 7] = (half_t)(seen & (1u << i) ? 1.0f : 0.0f);
+            for (int i = 0; i < 16; ++i) {
+                load_words<L::kVw>(vr[i], q + i * a.hd);
+                see[i >> 3][i & 7] = (half_t)(seen & (1u << i) ? 1.0f : 0.0f);
+            }
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+#pragma unroll
+                for (int w = 0; w < L::kVw; ++w)  // 0x38: one
+                    vr[i][w] = seen_by_any & (1u << i) ? 0x38383838u & (vbyte == 255 ? ~0u : nan_bytes(vr[i][w])) : 0u;
 #pragma unroll
             for (int j = 0; j < L::kD; j += 2) {
                 f4 n0 = f4{0, 0, 0, 0}, n1 = n0;
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    h8 even, odd, ne, no;
-                    v_pair<HD>(vr, k, j >> 2, (j >> 1) & 1, vscale, even, odd);
-                    split_nan(even, ne);
-                    split_nan(odd, no);
-                    o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p[k], o[j], 0, 0, 0);
-                    o[j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p[k], o[j + 1], 0, 0, 0);
-                    n0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(ne, see[k], n0, 0, 0, 0);
-                    n1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(no, see[k], n1, 0, 0, 0);
+                    h8 even, odd;
+                    v_pair<HD>(vr, k, j >> 2, (j >> 1) & 1, 1.0f, even, odd);
+                    n0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, see[k], n0, 0, 0, 0);
+                    n1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, see[k], n1, 0, 0, 0);
                 }
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -338,7 +377,8 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(Kv8Attn a) {
                 }
             }
         }
-        if (next < end) load_v(next);
+        load_v();
+        find_v(step + 2 * kWaves);
     }
 
     // the four waves' sums, joined
@@ -352,81 +392,96 @@ __global__ __launch_bounds__(256, 2) void kv8_attn_kernel(Kv8Attn a) {
 #pragma unroll
         for (int j = 0; j < L::kD; ++j) s_o[wave][col][(4 * grp + e) * L::kD + j] = o[j][e];
     __syncthreads();
-    const int64_t slot = a.first[g] + ((b * a.tiles[g] + tile) * a.Hkv + h) * a.nsplit[g] + split;
     const float inv_hd = 1.0f / static_cast<float>(a.hd);
+    const int64_t group = a.group0[g] + (b * a.tiles[g] + tile) * a.Hkv + h;
+    float* const part = a.part + (a.first[g] + ((b * a.tiles[g] + tile) * a.Hkv + h) * a.nsplit[g]) * kRows * (a.hd + 2);
+    const int64_t apart = static_cast<int64_t>(kRows) * (a.hd + 2);
+    const auto put = [&](int r, int d, float sum, float tot) {
+        const int rr = t.r0 + r, rs = rr / a.G;
+        const int64_t rp = t.sp + rs;
+        const bool rl = rp >= 0 && rp < t.sl && tot != 0.0f;
+        a.out[(tok0 + rs) * a.os + (h * a.G + rr - rs * a.G) * a.hd + d] = (half_t)(rl ? sum / tot : 0.0f);
+    };
     for (int i = threadIdx.x; i < t.rows * a.hd; i += 256) {
         const int r = small_div(i, inv_hd), d = i - r * a.hd;
         float mm = -INFINITY;
 #pragma unroll
         for (int w = 0; w < kWaves; ++w) mm = fmaxf(mm, s_ml[w][0][r]);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
         float sum = 0.0f, tot = 0.0f;
-        if (mm > -INFINITY) {
 #pragma unroll
-            for (int w = 0; w < kWaves; ++w) {
-                if (s_ml[w][0][r] == -INFINITY && s_ml[w][1][r] == 0.0f) continue;  // saw nothing
-                const float by = __builtin_amdgcn_exp2f(s_ml[w][0][r] - mm);
-                sum = fmaf(s_o[w][r][d], by, sum);
-                tot = fmaf(s_ml[w][1][r], by, tot);
-            }
-        } else {  // nothing seen, or NaN alone
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) tot += s_ml[w][1][r], sum += s_o[w][r][d];
+        for (int w = 0; w < kWaves; ++w) {  // a wave that saw nothing: exp2(-inf) = 0 of zeros
+            const float by = join_weight(s_ml[w][0][r], s_ml[w][1][r], ref);
+            sum = fmaf(s_o[w][r][d], by, sum);
+            tot = fmaf(s_ml[w][1][r], by, tot);
         }
-        const int rr = t.r0 + r, rs = rr / a.G;
-        const int64_t rp = t.sp + rs;
         if (t.used <= 1) {
-            const bool rl = rp >= 0 && rp < t.sl && tot != 0.0f;
-            a.out[(tok0 + rs) * a.os + (h * a.G + rr - rs * a.G) * a.hd + d] = (half_t)(rl ? sum / tot : 0.0f);
+            put(r, d, sum, tot);
         } else {
-            float* const p = a.part + (slot * kRows + r) * (a.hd + 2);
-            p[d] = sum;
+            float* const p = part + split * apart + r * (a.hd + 2);
+            store_agent(p + d, sum);
             if (d == 0) {
-                p[a.hd] = mm;
-                p[a.hd + 1] = tot;
+                store_agent(p + a.hd, mm);
+                store_agent(p + a.hd + 1, tot);
             }
         }
     }
-}
-
-// The splits of a tile, joined: one workgroup per (sequence, tile, KV head).
-__global__ __launch_bounds__(256) void kv8_join_kernel(Kv8Attn a) {
-    int64_t id = blockIdx.x;
-    int g = 0;
-    while (id >= a.group0[g + 1]) ++g;
-    id -= a.group0[g];
-    const int h = static_cast<int>(id % a.Hkv);
-    const int64_t bt = id / a.Hkv;
-    const int tile = static_cast<int>(bt % a.tiles[g]);
-    const int64_t b = bt / a.tiles[g];
-    const TileKeys t = tile_keys(a, g, b, tile);
     if (t.used <= 1) return;
-    const float* const part = a.part + (a.first[g] + (bt * a.Hkv + h) * a.nsplit[g]) * kRows * (a.hd + 2);
-    const int64_t step = static_cast<int64_t>(kRows) * (a.hd + 2);
-    for (int i = threadIdx.x; i < t.rows * a.hd; i += 256) {
-        const int r = i / a.hd, d = i - r * a.hd;
-        const float* const p = part + static_cast<int64_t>(r) * (a.hd + 2);
-        float mm = -INFINITY;
-        for (int s = 0; s < t.used; ++s) mm = fmaxf(mm, p[s * step + a.hd]);
-        float sum = 0.0f, tot = 0.0f;
-        for (int s = 0; s < t.used; ++s) {
-            const float ms = p[s * step + a.hd], ls = p[s * step + a.hd + 1];
-            if (ms == -INFINITY && ls == 0.0f) continue;
-            const float by = mm == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f(ms - mm);
-            sum = fmaf(p[s * step + d], by, sum);
-            tot = fmaf(ls, by, tot);
+    // The tile's last workgroup joins the splits, in their order.  The partial sums went through
+    // to memory and are read from there (agent scope), so no cache has to be written back.
+    __builtin_amdgcn_s_waitcnt(kDrainVmem);
+    __syncthreads();
+    unsigned* const counter = a.count + group - a.unsplit[g];
+    if (threadIdx.x == 0)
+        s_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
+                 static_cast<unsigned>(t.used - 1);
+    __syncthreads();
+    if (!s_last) return;
+    if (threadIdx.x == 0) *counter = 0;  // for the next call
+    float* const w_of = &s_o[0][0][0];   // [split][row], then the rows' sums
+    static_assert(kMaxSplits * kRows * 2 + kRows <= kWaves * kRows * (64 + 4), "the splits' weights fit");
+    float* const l_of = w_of + kMaxSplits * kRows;
+    for (int i = threadIdx.x; i < t.used * t.rows; i += 256) {
+        const int sp = i / t.rows, r = i - sp * t.rows;
+        w_of[sp * kRows + r] = load_agent(part + sp * apart + r * (a.hd + 2) + a.hd);
+        l_of[sp * kRows + r] = load_agent(part + sp * apart + r * (a.hd + 2) + a.hd + 1);
+    }
+    __syncthreads();
+    if (threadIdx.x < t.rows) {
+        const int r = threadIdx.x;
+        float mm = -INFINITY, tot = 0.0f;
+        for (int sp = 0; sp < t.used; ++sp) mm = fmaxf(mm, w_of[sp * kRows + r]);
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+        for (int sp = 0; sp < t.used; ++sp) {
+            const float l1 = l_of[sp * kRows + r], by = join_weight(w_of[sp * kRows + r], l1, ref);
+            w_of[sp * kRows + r] = by;
+            tot = fmaf(l1, by, tot);
         }
-        const int rr = t.r0 + r, rs = rr / a.G;
-        const int64_t rp = t.sp + rs;
-        const bool live = rp >= 0 && rp < t.sl && tot != 0.0f;
-        a.out[(a.sg.off[g] + b * t.S + rs) * a.os + (h * a.G + rr - rs * a.G) * a.hd + d] =
-            (half_t)(live ? sum / tot : 0.0f);
+        s_ml[0][0][r] = tot;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < t.rows * a.hd; i += 256) {
+        const int r = small_div(i, inv_hd), d = i - r * a.hd;
+        const float* const p = part + r * (a.hd + 2) + d;
+        float sum = 0.0f;
+        int sp = 0;
+        for (; sp + 8 <= t.used; sp += 8) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = load_agent(p + (sp + k) * apart);
+#pragma unroll
+            for (int k = 0; k < 8; ++k) sum = fmaf(v[k], w_of[(sp + k) * kRows + r], sum);
+        }
+        for (; sp < t.used; ++sp) sum = fmaf(load_agent(p + sp * apart), w_of[sp * kRows + r], sum);
+        put(r, d, sum, s_ml[0][0][r]);
     }
 }
 
-// Tiles, splits and slots of a call; what the launch and the workspace's size go by.
+// Tiles, splits and slots of a call; what the launch and the workspace's size go by.  A
+// segment of few (sequence, tile, KV head) is split over its keys.
 static int kv8_attn_plan(Kv8Attn& a, int64_t& slots) {
-    const int64_t kWant = 2048;  // workgroups that fill the GPU a few times over
     slots = 0;
+    int64_t unsplit = 0;
     for (int i = 0; i < a.sg.n; ++i) {
         const int64_t tiles = ceil_div(a.sg.S[i] * a.G, kRows);
         const int64_t groups = a.sg.B[i] * tiles * a.Hkv;
@@ -437,8 +492,14 @@ static int kv8_attn_plan(Kv8Attn& a, int64_t& slots) {
         a.first[i + 1] = a.first[i] + groups * ns;
         a.group0[i + 1] = a.group0[i] + groups;
         if (ns > 1) slots = a.first[i + 1];
+        else unsplit += groups;
+        a.unsplit[i] = unsplit;
     }
     return a.first[a.sg.n] <= kMaxGridX ? MI_OK : MI_ERR_UNSUPPORTED;
+}
+
+static int64_t kv8_attn_bytes(int64_t slots, int64_t hd) {
+    return slots > 0 ? kCounters * 4 + slots * kRows * (hd + 2) * 4 : 0;
 }
 
 static int kv8_attn_shape(int64_t T, int64_t Hq, int64_t Hkv, int64_t hd,
@@ -476,7 +537,7 @@ extern "C" int64_t mi_kv8_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int
     if (st != MI_OK) return st;
     const int pl = kv8_attn_plan(a, slots);
     if (pl != MI_OK) return pl;
-    return slots * kRows * (head_dim + 2) * 4;
+    return kv8_attn_bytes(slots, head_dim);
 }
 
 extern "C" int mi_kv8_attention_f16(const void* q, int64_t q_stride, const void* k_cache,
@@ -515,7 +576,7 @@ extern "C" int mi_kv8_attention_f16(const void* q, int64_t q_stride, const void*
     int64_t slots = 0;
     const int pl = kv8_attn_plan(a, slots);
     if (pl != MI_OK) return pl;
-    const int64_t need = slots * kRows * (head_dim + 2) * 4;
+    const int64_t need = kv8_attn_bytes(slots, head_dim);
     if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return MI_ERR_INVALID_ARGUMENT;
     const void* bufs[6] = {k_cache, v_cache, k_scale, v_scale, q, workspace};
     const int64_t lens[6] = {cells * block_size * head_dim, cells * block_size * head_dim, cells, cells, qb, need};
@@ -535,12 +596,12 @@ extern "C" int mi_kv8_attention_f16(const void* q, int64_t q_stride, const void*
     a.num_blocks = num_blocks;
     a.window = static_cast<int>(std::min<int64_t>(window, int64_t{1} << 30));
     a.c = scale * 1.4426950408889634f;
-    a.part = static_cast<float*>(workspace);
+    a.count = static_cast<unsigned*>(workspace);
+    a.part = static_cast<float*>(workspace) + kCounters;
     const hipStream_t s = as_stream(stream);
     const dim3 grid(static_cast<unsigned>(a.first[a.sg.n])), block(256);
     if (head_dim <= 64) kv8_attn_kernel<64><<<grid, block, 0, s>>>(a);
     else if (head_dim <= 128) kv8_attn_kernel<128><<<grid, block, 0, s>>>(a);
     else kv8_attn_kernel<256><<<grid, block, 0, s>>>(a);
-    if (slots > 0) kv8_join_kernel<<<dim3(static_cast<unsigned>(a.group0[a.sg.n])), block, 0, s>>>(a);
     return launch_status();
 }

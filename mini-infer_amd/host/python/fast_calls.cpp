@@ -23,9 +23,11 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/ops/empty.h>
 #include <ATen/ops/empty_like.h>
+#include <c10/hip/HIPFunctions.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <cmath>
 #include <vector>
 
 #include "mi_chain.h"
@@ -462,6 +464,277 @@ MI_FAST(embedding_rmsnorm) {
     });
 }
 
+// --- rotary positions in other layouts, the 8-bit cache, its pages ------------------
+
+// A call goes to a stream of the current device: so must its tensors.
+const at::Tensor& here(const at::Tensor& t) {
+    need(t.device().index() == c10::hip::current_device());
+    return t;
+}
+
+// q, k, ... [T, H, hd] fp16, each token a contiguous row, any distance apart.
+struct TokenRows {
+    const at::Tensor* t = nullptr;
+    int64_t T = 0, H = 0, hd = 0, stride = 0;
+    explicit TokenRows(PyObject* o) {
+        if (o == Py_None) return;
+        need(THPVariable_CheckExact(o));
+        t = &THPVariable_Unpack(o);
+        need(t->is_cuda() && t->scalar_type() == at::kHalf && t->dim() == 3);
+        here(*t);
+        T = t->size(0);
+        H = t->size(1);
+        hd = t->size(2);
+        need(t->numel() > 0);
+        need((hd == 1 || t->stride(2) == 1) && (H == 1 || t->stride(1) == hd));
+        stride = T > 1 ? t->stride(0) : H * hd;
+        need(stride >= H * hd);
+    }
+    bool like(const TokenRows& o) const { return T == o.T && H == o.H && hd == o.hd; }
+    void* p() const { return t ? ptr(*t) : nullptr; }
+};
+
+// (q, k or None, positions, inv_freq, interleaved, mscale, q_out or None, k_out or None, stream)
+MI_FAST(rope_partial_qk) {
+    return guarded(n, 9, [&] {
+        const TokenRows q(a[0]), k(a[1]);
+        PyObject *qo_ = a[6] == Py_None ? a[0] : a[6], *ko_ = a[7] == Py_None ? a[1] : a[7];
+        const TokenRows qo(qo_), ko(ko_);
+        const auto& pos = here(tensor(a[2], at::kLong));
+        const Floats inv(a[3]);
+        need(q.t && qo.like(q) && ko.like(k) && pos.numel() == q.T && inv.view.ndim == 1);
+        need((!k.t || (k.T == q.T && k.hd == q.hd)) && inv.size() > 0 && 2 * inv.size() <= q.hd);
+        const int inter = truth(a[4]);
+        const float m = static_cast<float>(number(a[5]));
+        void* s = stream_of(a[8]);
+        MI_CALL(mi_rope_partial_qk_f16, q.p(), k.p(), qo.p(), ko.p(), static_cast<const int64_t*>(ptr(pos)),
+                inv.data(), q.T, q.H, k.H, q.hd, 2 * inv.size(), q.stride, k.stride, qo.stride, ko.stride,
+                inter, m, s);
+        return PyTuple_Pack(2, qo_, ko_);
+    });
+}
+
+// k_cache, v_cache [L, num_blocks, Hkv, bs, hd] and their scales, on the current device
+struct Kv8Cache {
+    const at::Tensor &k, &v, &ks, &vs;
+    int64_t L, NB, H, bs, hd;
+    explicit Kv8Cache(PyObject* const* a)
+        : k(here(tensor(a[0], at::kFloat8_e4m3fn))),
+          v(here(tensor(a[1], at::kFloat8_e4m3fn))),
+          ks(here(tensor(a[2], at::kByte))),
+          vs(here(tensor(a[3], at::kByte))) {
+        need(k.dim() == 5 && v.sizes() == k.sizes() && ks.sizes() == k.sizes().slice(0, 3) &&
+             vs.sizes() == ks.sizes());
+        L = k.size(0);
+        NB = k.size(1);
+        H = k.size(2);
+        bs = k.size(3);
+        hd = k.size(4);
+    }
+};
+
+// The segments of a call: dicts in a list.
+struct Segments {
+    static constexpr int kMost = 8;
+    mi_kv_segment g[kMost];
+    int n = 0;
+    explicit Segments(PyObject* o) {
+        static PyObject* const names[5] = {
+            PyUnicode_InternFromString("token_offset"), PyUnicode_InternFromString("S"),
+            PyUnicode_InternFromString("block_table"), PyUnicode_InternFromString("seq_len"),
+            PyUnicode_InternFromString("start_pos")};
+        need(PyList_CheckExact(o) && PyList_GET_SIZE(o) <= kMost);
+        for (n = 0; n < PyList_GET_SIZE(o); ++n) {
+            PyObject* d = PyList_GET_ITEM(o, n);
+            need(PyDict_CheckExact(d));
+            PyObject* v[5];
+            for (int i = 0; i < 5; ++i) {
+                v[i] = PyDict_GetItemWithError(d, names[i]);  // borrowed
+                if (!v[i]) {
+                    PyErr_Clear();
+                    throw Leave{};
+                }
+            }
+            const auto &bt = here(tensor(v[2], at::kInt)), &sl = here(tensor(v[3], at::kInt)),
+                       &sp = here(tensor(v[4], at::kInt));
+            need(bt.dim() == 2 && sl.numel() == bt.size(0) && sp.numel() == bt.size(0));
+            g[n] = {whole(v[0]), bt.size(0), whole(v[1]), static_cast<const int*>(ptr(bt)),
+                    static_cast<const int*>(ptr(sl)), static_cast<const int*>(ptr(sp)), bt.size(1)};
+        }
+    }
+};
+
+// (k, v, k_cache, v_cache, k_scale, v_scale, layer, segments, stream)
+MI_FAST(kv8_scatter) {
+    return guarded(n, 9, [&] {
+        const TokenRows k(a[0]), v(a[1]);
+        const Kv8Cache c(a + 2);
+        const int64_t layer = whole(a[6]);
+        const Segments sg(a[7]);
+        need(k.t && v.like(k) && k.H == c.H && k.hd == c.hd && layer >= 0 && layer < c.L);
+        void* s = stream_of(a[8]);
+        MI_CALL(mi_kv8_scatter_f16, k.p(), v.p(), k.stride, v.stride, k.T, k.H, k.hd, ptr(c.k), ptr(c.v),
+                ptr(c.ks), ptr(c.vs), layer, c.NB, c.bs, sg.g, sg.n, s);
+        return PyTuple_Pack(2, a[2], a[3]);
+    });
+}
+
+// (q, k_cache, v_cache, k_scale, v_scale, layer, segments, scale or None, window, out, workspace, stream)
+MI_FAST(kv8_attention) {
+    return guarded(n, 12, [&] {
+        const TokenRows q(a[0]), out(a[9]);
+        const Kv8Cache c(a + 1);
+        const int64_t layer = whole(a[5]);
+        const Segments sg(a[6]);
+        need(q.t && out.t && out.like(q) && q.hd == c.hd && c.H > 0 && q.H % c.H == 0 && layer >= 0 &&
+             layer < c.L);
+        const float scale = static_cast<float>(a[7] == Py_None ? 1.0 / std::sqrt(static_cast<double>(q.hd))
+                                                               : number(a[7]));
+        const int64_t window = whole(a[8]);
+        const auto& w = here(bytes_on_gpu(a[10]));
+        void* s = stream_of(a[11]);
+        MI_CALL(mi_kv8_attention_f16, q.p(), q.stride, ptr(c.k), ptr(c.v), ptr(c.ks), ptr(c.vs), out.p(),
+                out.stride, q.T, q.H, c.H, q.hd, scale, window, layer, c.NB, c.bs, sg.g, sg.n, ptr(w),
+                static_cast<int64_t>(w.nbytes()), s);
+        Py_INCREF(a[9]);
+        return a[9];
+    });
+}
+
+// The tensors of a cache, [L, num_blocks, ...] each.
+struct PageTensors {
+    static constexpr int kMost = 8;
+    mi_kv_pages g[kMost];
+    int n = 0;
+    int64_t NB = 0;
+    explicit PageTensors(PyObject* o) {
+        const bool list = PyList_CheckExact(o);
+        need(list || PyTuple_CheckExact(o));
+        const Py_ssize_t m = list ? PyList_GET_SIZE(o) : PyTuple_GET_SIZE(o);
+        need(m > 0 && m <= kMost);
+        for (n = 0; n < m; ++n) {
+            const auto& t = here(bytes_on_gpu(list ? PyList_GET_ITEM(o, n) : PyTuple_GET_ITEM(o, n)));
+            need(t.dim() >= 2 && t.numel() > 0);
+            if (n == 0) NB = t.size(1);
+            need(t.size(1) == NB);
+            g[n] = {ptr(t), t.size(0), static_cast<int64_t>(t.nbytes()) / (t.size(0) * NB)};
+        }
+    }
+};
+
+const at::Tensor& ints(PyObject* o) { return here(tensor(o, at::kInt)); }
+int* ip(const at::Tensor& t) { return static_cast<int*>(ptr(t)); }
+
+// block_table [B, mb], seq_len [B], ref_count [num_blocks]
+struct PageTable {
+    const at::Tensor &table, &seq, &ref;
+    PageTable(PyObject* t, PyObject* s, PyObject* r) : table(ints(t)), seq(ints(s)), ref(ints(r)) {
+        need(table.dim() == 2 && seq.numel() == table.size(0));
+    }
+    int64_t B() const { return table.size(0); }
+    int64_t mb() const { return table.size(1); }
+    int64_t NB() const { return ref.numel(); }
+};
+
+// A workspace: the caller's, or a new one (the current stream's: a call on another
+// stream is left to the wrapper, which tells the allocator).
+struct Scratch {
+    at::Tensor made;
+    const at::Tensor* t;
+    Scratch(PyObject* o, int64_t bytes, const at::Tensor& on, PyObject* stream) {
+        need(bytes > 0);
+        if (o == Py_None) {
+            need(stream == Py_None);
+            made = at::empty({(bytes + 3) / 4}, on.options().dtype(at::kInt));
+        }
+        t = o == Py_None ? &made : &here(bytes_on_gpu(o));
+    }
+    int64_t bytes() const { return static_cast<int64_t>(t->nbytes()); }
+};
+
+// (caches, src, dst, status or None, stream)
+MI_FAST(kv_copy_pages) {
+    return guarded(n, 5, [&] {
+        const PageTensors c(a[0]);
+        const auto &src = ints(a[1]), &dst = ints(a[2]);
+        const int64_t m = src.numel();
+        need(dst.numel() == m);
+        const Out status(a[3], src, at::kInt, {m});
+        need(status.t->numel() == m);
+        here(*status.t);
+        void* s = stream_of(a[4]);
+        MI_CALL(mi_kv_pages_copy, c.g, c.n, c.NB, ip(src), ip(dst), m, ip(*status.t), s);
+        return status.result();
+    });
+}
+
+// (block_table, seq_len, ref_count, rows, stream): True where the call was made
+MI_FAST(kv_free) {
+    return guarded(n, 5, [&] {
+        const PageTable p(a[0], a[1], a[2]);
+        const auto& rows = ints(a[3]);
+        void* s = stream_of(a[4]);
+        MI_CALL(mi_kv_pages_free, ip(p.table), ip(p.seq), ip(p.ref), p.B(), p.mb(), p.NB(), ip(rows),
+                rows.numel(), s);
+        Py_RETURN_TRUE;
+    });
+}
+
+// (block_table, seq_len, ref_count, parents, children, status or None, stream)
+MI_FAST(kv_fork) {
+    return guarded(n, 7, [&] {
+        const PageTable p(a[0], a[1], a[2]);
+        const auto &from = ints(a[3]), &to = ints(a[4]);
+        const int64_t m = from.numel();
+        need(to.numel() == m);
+        const Out status(a[5], from, at::kInt, {m});
+        need(status.t->numel() == m);
+        here(*status.t);
+        void* s = stream_of(a[6]);
+        MI_CALL(mi_kv_pages_fork, ip(p.table), ip(p.seq), ip(p.ref), p.B(), p.mb(), p.NB(), ip(from), ip(to),
+                m, ip(*status.t), s);
+        return status.result();
+    });
+}
+
+// (caches, block_table, seq_len, ref_count, rows, lengths, block_size, status or None,
+// workspace or None, stream)
+MI_FAST(kv_reserve) {
+    return guarded(n, 10, [&] {
+        const PageTensors c(a[0]);
+        const PageTable p(a[1], a[2], a[3]);
+        const auto &rows = ints(a[4]), &lens = ints(a[5]);
+        const int64_t m = rows.numel(), bs = whole(a[6]);
+        need(lens.numel() == m && c.NB == p.NB());
+        const Out status(a[7], rows, at::kInt, {m});
+        need(status.t->numel() == m);
+        here(*status.t);
+        const Scratch w(a[8], mi_kv_pages_workspace_bytes(p.NB(), m), p.table, a[9]);
+        void* s = stream_of(a[9]);
+        MI_CALL(mi_kv_pages_reserve, c.g, c.n, ip(p.table), ip(p.seq), ip(p.ref), p.B(), p.mb(), p.NB(), bs,
+                ip(rows), ip(lens), m, ip(*status.t), ptr(*w.t), w.bytes(), s);
+        return status.result();
+    });
+}
+
+// (caches, block_table, ref_count, moved or None, workspace or None, stream)
+MI_FAST(kv_compact) {
+    return guarded(n, 6, [&] {
+        const PageTensors c(a[0]);
+        const auto &table = ints(a[1]), &ref = ints(a[2]);
+        const int64_t NB = ref.numel();
+        need(table.dim() == 2 && c.NB == NB);
+        const Out moved(a[3], ref, at::kInt, {NB});
+        need(moved.t->numel() == NB);
+        here(*moved.t);
+        const Scratch w(a[4], mi_kv_pages_workspace_bytes(NB, 0), table, a[5]);
+        void* s = stream_of(a[5]);
+        MI_CALL(mi_kv_pages_compact, c.g, c.n, ip(table), ip(ref), table.size(0), table.size(1), NB,
+                ip(*moved.t), ptr(*w.t), w.bytes(), s);
+        return moved.result();
+    });
+}
+
 // (address of an mi_chain_desc, last_stage, stream): the call's status.
 MI_FAST(chain_run) {
     if (n != 3) {
@@ -511,6 +784,14 @@ PyMethodDef methods[] = {MI_METHOD(rmsnorm),
                          MI_METHOD(rope_tables),
                          MI_METHOD(embedding_gather),
                          MI_METHOD(embedding_rmsnorm),
+                         MI_METHOD(rope_partial_qk),
+                         MI_METHOD(kv8_scatter),
+                         MI_METHOD(kv8_attention),
+                         MI_METHOD(kv_copy_pages),
+                         MI_METHOD(kv_free),
+                         MI_METHOD(kv_fork),
+                         MI_METHOD(kv_reserve),
+                         MI_METHOD(kv_compact),
                          MI_METHOD(chain_run),
                          {"current_stream", current_stream, METH_NOARGS, nullptr},
                          {nullptr, nullptr, 0, nullptr}};

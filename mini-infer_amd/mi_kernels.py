@@ -985,6 +985,10 @@ def rope_partial_qk(q, k, positions, inv_freq, interleaved: bool = False, mscale
     first 2 * len(inv_freq) elements of each head, as halves or as interleaved
     pairs, cos and sin times mscale; tokens may be any distance apart (slices of
     a fused QKV product).  In place, or into q_out / k_out.  Returns (q_out, k_out)."""
+    r = (_fast or _load_fast()).rope_partial_qk(q, k, positions, inv_freq, interleaved, mscale, q_out,
+                                                k_out, stream)
+    if r is not None:
+        return r
     torch = _torch()
     qs = _need_rows(q, "q")
     T, Hq, hd = q.shape
@@ -1065,6 +1069,10 @@ def kv8_scatter(k, v, k_cache, v_cache, k_scale, v_scale, layer: int, segments, 
     (kv8_cache) for the tokens of `segments` (as rope_kv_scatter's): each page and head
     takes the least power-of-two scale that holds its largest value; see
     mi_kv8_scatter_f16."""
+    r = (_fast or _load_fast()).kv8_scatter(k, v, k_cache, v_cache, k_scale, v_scale, layer, segments,
+                                            stream)
+    if r is not None:
+        return r
     L, NB, Hkv, bs, hd = _kv8_checks(k_cache, v_cache, k_scale, v_scale, layer, k)
     ks, vs = _need_rows(k, "k"), _need_rows(v, "v")
     T = k.shape[0]
@@ -1095,6 +1103,10 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, layer: int, segments, s
     zeros where no segment has the token.  `workspace`
     (kv8_attention_workspace_bytes) must be zero before its first use and kept for
     this function; without one, a call makes its own.  Returns out."""
+    r = (_fast or _load_fast()).kv8_attention(q, k_cache, v_cache, k_scale, v_scale, layer, segments,
+                                              scale, window, out, workspace, stream)
+    if r is not None:
+        return r
     torch = _torch()
     qs = _need_rows(q, "q")
     T, Hq, hd = q.shape
@@ -1205,6 +1217,9 @@ def kv_copy_pages(caches, src, dst, status=None, stream=None):
     num_blocks, ...], any type) and layer.  Returns status [n]: KV_DONE, or KV_REFUSED
     for a pair whose pages lie outside or whose dst is another pair's src or an
     earlier pair's dst."""
+    r = (_fast or _load_fast()).kv_copy_pages(caches, src, dst, status, stream)
+    if r is not None:
+        return r
     if not caches:
         raise ValueError("caches must hold at least one tensor")
     _page_ints(src, (src, "src"), (dst, "dst"))
@@ -1222,6 +1237,8 @@ def kv_copy_pages(caches, src, dst, status=None, stream=None):
 
 def kv_free(block_table, seq_len, ref_count, rows, stream=None):
     """Rows `rows` (int32) of block_table [B, max_blocks] give up their pages and become empty."""
+    if (_fast or _load_fast()).kv_free(block_table, seq_len, ref_count, rows, stream) is not None:
+        return
     B, mb, NB = _page_state(block_table, seq_len, ref_count)
     _page_ints(block_table, (rows, "rows"))
     _check(load_library().mi_kv_pages_free(_ptr(block_table), _ptr(seq_len), _ptr(ref_count), B, mb,
@@ -1232,6 +1249,10 @@ def kv_free(block_table, seq_len, ref_count, rows, stream=None):
 def kv_fork(block_table, seq_len, ref_count, parents, children, status=None, stream=None):
     """Row children[i], which has to be empty, comes to share all pages of row parents[i].  Returns
     status [n] (KV_DONE or KV_REFUSED)."""
+    r = (_fast or _load_fast()).kv_fork(block_table, seq_len, ref_count, parents, children, status,
+                                        stream)
+    if r is not None:
+        return r
     B, mb, NB = _page_state(block_table, seq_len, ref_count)
     _page_ints(block_table, (parents, "parents"), (children, "children"))
     n = parents.numel()
@@ -1249,6 +1270,10 @@ def kv_reserve(caches, block_table, seq_len, ref_count, rows, lengths, block_siz
     """Row rows[i] grows to lengths[i] tokens: new pages, and a copy of its last page in all caches
     where that is partly full and shared.  Returns status [n] (KV_DONE, KV_FULL where
     the free pages did not reach, KV_REFUSED)."""
+    r = (_fast or _load_fast()).kv_reserve(caches, block_table, seq_len, ref_count, rows, lengths,
+                                           block_size, status, workspace, stream)
+    if r is not None:
+        return r
     B, mb, NB = _page_state(block_table, seq_len, ref_count)
     _page_ints(block_table, (rows, "rows"), (lengths, "lengths"))
     n = rows.numel()
@@ -1267,6 +1292,9 @@ def kv_reserve(caches, block_table, seq_len, ref_count, rows, lengths, block_siz
 def kv_compact(caches, block_table, ref_count, moved=None, workspace=None, stream=None):
     """Moves the live pages to the front of the cache, in all caches, in ref_count and in the
     table.  Returns moved [num_blocks]: each page's new place, -1 for one that was free."""
+    r = (_fast or _load_fast()).kv_compact(caches, block_table, ref_count, moved, workspace, stream)
+    if r is not None:
+        return r
     B, mb, NB = _page_state(block_table, None, ref_count)
     arr = _page_caches(caches, NB, block_table)
     moved = _status(moved, NB, block_table)
