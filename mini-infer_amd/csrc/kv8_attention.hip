@@ -18,107 +18,18 @@
 #include <algorithm>
 #include <cmath>
 
-#include "kv8.h"
+#include "kv8_attn.h"
 #include "mi_host.h"
 
 namespace mi {
 
-typedef float f4 __attribute__((ext_vector_type(4)));
-
+constexpr int kFewRows = 64;   // query rows of a (sequence, KV head) up to which tiles of 16 take them
 constexpr int kRows = 16;      // query rows of a tile: (token, head of the KV head's group)
 constexpr int kKeys = 64;      // keys of a wave's step
 constexpr int kWaves = 4;      // waves of a workgroup, each on every fourth step
-constexpr float kPShift = 14.0f;
-constexpr int kMaxSplits = 64;
-constexpr int64_t kWant = 2048;                  // workgroups that a segment is split into at most
-constexpr int64_t kCounters = kKv8Segs * kWant;  // at the head of the workspace, zeros between calls
-
-struct Kv8Attn {
-    const half_t* q;
-    half_t* out;
-    const uint8_t *kc, *vc, *ks, *vs;
-    int64_t qs, os, num_blocks, layer;
-    int Hq, Hkv, G, hd, bs, window;
-    float c;  // scale * log2(e)
-    float* part;  // [slot][row][hd + 2]: sums, then maximum and sum of weights
-    unsigned* count;  // splits done, per (sequence, tile, KV head) of the segments in splits
-    int64_t unsplit[kKv8Segs];  // such groups of the segments before that are in none
-    Kv8Segs sg;
-    int tiles[kKv8Segs], nsplit[kKv8Segs];
-    int64_t first[kKv8Segs + 1];  // a segment's first workgroup, and its first slot
-    int64_t group0[kKv8Segs + 1]; // a segment's first (sequence, tile, KV head)
-};
-
-// What a tile of rows attends to.
-struct TileKeys {
-    int S, r0, rows;       // the sequence's tokens; first row, rows of the tile
-    int64_t sp, sl;        // the sequence's start position and length
-    int64_t lo, hi;        // keys that some live row sees
-    int64_t base;          // lo, down to a block of 16
-    int steps, per, used;  // steps of 64 keys from base; steps of a split, splits in use
-};
-
-__device__ __forceinline__ TileKeys tile_keys(const Kv8Attn& a, int g, int64_t b, int tile) {
-    TileKeys t;
-    t.S = static_cast<int>(a.sg.S[g]);
-    t.r0 = tile * kRows;
-    const int all = t.S * a.G;
-    t.rows = min(kRows, all - t.r0);
-    t.sp = a.sg.sp[g][b];
-    t.sl = a.sg.sl[g][b];
-    const int64_t first = max<int64_t>(t.sp + t.r0 / a.G, 0);
-    const int64_t last = min(t.sp + (t.r0 + t.rows - 1) / a.G, t.sl - 1);
-    t.hi = min<int64_t>(last + 1, a.sg.mb[g] * a.bs);
-    t.lo = a.window > 0 ? max<int64_t>(first - a.window + 1, 0) : 0;
-    if (last < first) t.hi = t.lo = 0;
-    t.base = t.lo & ~int64_t{15};
-    t.steps = t.hi > t.lo && a.num_blocks > 0 ? static_cast<int>((t.hi - t.base + kKeys - 1) / kKeys) : 0;
-    const int ns = a.nsplit[g];
-    t.per = max((t.steps + ns - 1) / ns, kWaves);
-    t.per = (t.per + kWaves - 1) / kWaves * kWaves;
-    t.used = (t.steps + t.per - 1) / t.per;
-    return t;
-}
-
-// id % d; id becomes id / d.
-__device__ __forceinline__ int divmod(uint32_t& id, int d) {
-    const uint32_t q = id / static_cast<uint32_t>(d), r = id - q * static_cast<uint32_t>(d);
-    id = q;
-    return static_cast<int>(r);
-}
-
-__device__ __forceinline__ float max_over_groups(float v) {
-    uint32_t a, b;
-    pair_xor16(__builtin_bit_cast(uint32_t, v), a, b);
-    v = fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
-    pair_xor32(__builtin_bit_cast(uint32_t, v), a, b);
-    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
-}
-__device__ __forceinline__ float sum_over_groups(float v) {
-    v += __shfl_xor(v, 16, kWave);
-    return v + __shfl_xor(v, 32, kWave);
-}
-
-// What a partial sum with maximum m and sum of weights l counts, beside the maximum ref;
-// one that saw nothing counts nothing, and one of NaN alone (m stays -inf) must not be lost.
-__device__ __forceinline__ float join_weight(float m, float l, float ref) {
-    return m == -INFINITY ? (l == 0.0f ? 0.0f : 1.0f) : __builtin_amdgcn_exp2f(m - ref);
-}
-
-__device__ __forceinline__ void store_agent(float* p, float v) {
-    __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-__device__ __forceinline__ float load_agent(const float* p) {
-    return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
-}
-
-template <int W>
-__device__ __forceinline__ void load_words(uint32_t* to, const uint8_t* p) {
-    typedef uint32_t vec __attribute__((ext_vector_type(W)));
-    const vec v = *reinterpret_cast<const vec*>(p);
-#pragma unroll
-    for (int i = 0; i < W; ++i) to[i] = v[i];
-}
+constexpr int64_t kWant = 2048;        // workgroups that a segment of few rows is split into
+constexpr int64_t kPromptWant = 512;   // and one of many rows
+constexpr int64_t kCounters = kKv8Segs * kWant / 2;  // at the head of the workspace, zeros between calls
 
 template <int HD>
 struct Tile {
@@ -153,12 +64,6 @@ __device__ __forceinline__ void v_pair(const uint32_t (&raw)[16][Tile<HD>::kVw],
     odd = __builtin_bit_cast(h8, u4{o[0], o[1], o[2], o[3]});
 }
 
-// All bits of the bytes of w that are NaN.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
-    const uint32_t top = ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
-    return top | (top - (top >> 7));
-}
-
 // One workgroup: a tile of 16 rows of one sequence and KV head, over one split of its keys.
 // A wave's step of 64 keys: K's bytes to fp16 and the scores; the softmax's step; V's bytes
 // to fp16, transposed in pairs by byte permutes, and the sums.  K of the next step is
@@ -180,7 +85,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
     const int split = divmod(id, a.nsplit[g]);
     const int tile = divmod(id, a.tiles[g]);
     const int64_t b = id;
-    const TileKeys t = tile_keys(a, g, b, tile);
+    const TileKeys t = tile_keys<kRows, kKeys, kWaves>(a, g, b, tile);
     if (split >= max(t.used, 1)) return;
     const int col = lane & 15, grp = lane >> 4;
     const int64_t tok0 = a.sg.off[g] + b * t.S;
@@ -197,6 +102,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
         const int d = grp * (HD / 4) + i * 8;
         qf[i] = h8(0);
         if (live && d < a.hd) qf[i] = ld8(a.q + (tok0 + s) * a.qs + head * a.hd + d);
+        if (a.neg) qf[i] = -qf[i];
     }
 
     // The page of a 16-key block, -1 where it has none.  Every load is unconditional --
@@ -393,8 +299,9 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
         for (int j = 0; j < L::kD; ++j) s_o[wave][col][(4 * grp + e) * L::kD + j] = o[j][e];
     __syncthreads();
     const float inv_hd = 1.0f / static_cast<float>(a.hd);
-    const int64_t group = a.group0[g] + (b * a.tiles[g] + tile) * a.Hkv + h;
-    float* const part = a.part + (a.first[g] + ((b * a.tiles[g] + tile) * a.Hkv + h) * a.nsplit[g]) * kRows * (a.hd + 2);
+    const int64_t group = (b * a.tiles[g] + tile) * a.Hkv + h;
+    // [split][row][hd + 2]: sums, then the maximum and the sum of the weights
+    float* const part = a.part + a.part0[g] + group * a.nsplit[g] * kRows * (a.hd + 2);
     const int64_t apart = static_cast<int64_t>(kRows) * (a.hd + 2);
     const auto put = [&](int r, int d, float sum, float tot) {
         const int rr = t.r0 + r, rs = rr / a.G;
@@ -431,7 +338,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
     // to memory and are read from there (agent scope), so no cache has to be written back.
     __builtin_amdgcn_s_waitcnt(kDrainVmem);
     __syncthreads();
-    unsigned* const counter = a.count + group - a.unsplit[g];
+    unsigned* const counter = a.count + a.cnt0[g] + group;
     if (threadIdx.x == 0)
         s_last = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) ==
                  static_cast<unsigned>(t.used - 1);
@@ -477,29 +384,41 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
     }
 }
 
-// Tiles, splits and slots of a call; what the launch and the workspace's size go by.  A
-// segment of few (sequence, tile, KV head) is split over its keys.
-static int kv8_attn_plan(Kv8Attn& a, int64_t& slots) {
-    slots = 0;
-    int64_t unsplit = 0;
-    for (int i = 0; i < a.sg.n; ++i) {
-        const int64_t tiles = ceil_div(a.sg.S[i] * a.G, kRows);
-        const int64_t groups = a.sg.B[i] * tiles * a.Hkv;
-        const int64_t ns = std::clamp<int64_t>(kWant / std::max<int64_t>(groups, 1), 1,
-                                               std::min<int64_t>(a.sg.mb[i], kMaxSplits));
-        a.tiles[i] = static_cast<int>(tiles);
-        a.nsplit[i] = static_cast<int>(ns);
-        a.first[i + 1] = a.first[i] + groups * ns;
-        a.group0[i + 1] = a.group0[i] + groups;
-        if (ns > 1) slots = a.first[i + 1];
-        else unsplit += groups;
-        a.unsplit[i] = unsplit;
+// The segments of a call, those of few query rows in `few` and the others in `many`, with
+// their tiles and splits (a segment of few tiles is split over its keys) and what they need of the
+// workspace.  By the segments' B, S and table width alone.
+static int kv8_attn_plan(const Kv8Attn& all, Kv8Attn& few, Kv8Attn& many, int64_t& bytes) {
+    few = many = all;
+    few.sg.n = many.sg.n = 0;
+    int64_t floats = 0, counters = 0;
+    for (int i = 0; i < all.sg.n; ++i) {
+        const int64_t rows = all.sg.S[i] * all.G;
+        const bool wide = rows > kFewRows;
+        Kv8Attn& a = wide ? many : few;
+        const int n = a.sg.n++;
+        a.sg.off[n] = all.sg.off[i];
+        a.sg.B[n] = all.sg.B[i];
+        a.sg.S[n] = all.sg.S[i];
+        a.sg.mb[n] = all.sg.mb[i];
+        a.sg.bt[n] = all.sg.bt[i];
+        a.sg.sl[n] = all.sg.sl[i];
+        a.sg.sp[n] = all.sg.sp[i];
+        const int64_t tile = wide ? kPromptRows : kRows, tiles = ceil_div(rows, tile);
+        const int64_t groups = a.sg.B[n] * tiles * a.Hkv;
+        const int64_t ns = std::clamp<int64_t>((wide ? kPromptWant : kWant) / std::max<int64_t>(groups, 1), 1,
+                                               std::min<int64_t>(a.sg.mb[n], kMaxSplits));
+        a.tiles[n] = static_cast<int>(tiles);
+        a.nsplit[n] = static_cast<int>(ns);
+        a.first[n + 1] = a.first[n] + groups * ns;
+        a.part0[n] = floats;
+        a.cnt0[n] = counters;
+        if (ns > 1) {
+            floats += groups * ns * tile * (a.hd + 2);
+            counters += groups;
+        }
     }
-    return a.first[a.sg.n] <= kMaxGridX ? MI_OK : MI_ERR_UNSUPPORTED;
-}
-
-static int64_t kv8_attn_bytes(int64_t slots, int64_t hd) {
-    return slots > 0 ? kCounters * 4 + slots * kRows * (hd + 2) * 4 : 0;
+    bytes = floats > 0 ? 4 * (kCounters + floats) : 0;
+    return few.first[few.sg.n] <= kMaxGridX && many.first[many.sg.n] <= kMaxGridX ? MI_OK : MI_ERR_UNSUPPORTED;
 }
 
 static int kv8_attn_shape(int64_t T, int64_t Hq, int64_t Hkv, int64_t hd,
@@ -525,8 +444,8 @@ static int kv8_attn_shape(int64_t T, int64_t Hq, int64_t Hkv, int64_t hd,
 extern "C" int64_t mi_kv8_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t head_dim,
                                                     const mi_kv_segment* segments, int num_segments) {
     using namespace mi;
-    Kv8Attn a{};
-    int64_t slots = 0, T = 0;
+    Kv8Attn a{}, few, many;
+    int64_t bytes = 0, T = 0;
     for (int i = 0; i < num_segments && segments; ++i) {  // any packing of the segments
         const mi_kv_segment& g = segments[i];
         if (g.B > 0 && g.S > 0 && g.B < (int64_t{1} << 31) && g.S < (int64_t{1} << 31) && g.token_offset >= 0 &&
@@ -535,9 +454,8 @@ extern "C" int64_t mi_kv8_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int
     }
     const int st = kv8_attn_shape(T, Hq, Hkv, head_dim, segments, num_segments, a);
     if (st != MI_OK) return st;
-    const int pl = kv8_attn_plan(a, slots);
-    if (pl != MI_OK) return pl;
-    return kv8_attn_bytes(slots, head_dim);
+    const int pl = kv8_attn_plan(a, few, many, bytes);
+    return pl != MI_OK ? pl : bytes;
 }
 
 extern "C" int mi_kv8_attention_f16(const void* q, int64_t q_stride, const void* k_cache,
@@ -573,17 +491,6 @@ extern "C" int mi_kv8_attention_f16(const void* q, int64_t q_stride, const void*
         return MI_ERR_UNSUPPORTED;
     const int64_t cells = (layer + 1) * num_blocks * Hkv;
     const int64_t qb = 2 * ((T - 1) * q_stride + row), ob = 2 * ((T - 1) * out_stride + row);
-    int64_t slots = 0;
-    const int pl = kv8_attn_plan(a, slots);
-    if (pl != MI_OK) return pl;
-    const int64_t need = kv8_attn_bytes(slots, head_dim);
-    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return MI_ERR_INVALID_ARGUMENT;
-    const void* bufs[6] = {k_cache, v_cache, k_scale, v_scale, q, workspace};
-    const int64_t lens[6] = {cells * block_size * head_dim, cells * block_size * head_dim, cells, cells, qb, need};
-    for (int i = 0; i < 6; ++i) {
-        if (overlaps(bufs[i], lens[i], out, ob)) return MI_ERR_ALIASING;
-        if (i < 5 && overlaps(bufs[i], lens[i], workspace, need)) return MI_ERR_ALIASING;
-    }
     a.q = static_cast<const half_t*>(q);
     a.out = static_cast<half_t*>(out);
     a.kc = static_cast<const uint8_t*>(k_cache);
@@ -595,13 +502,28 @@ extern "C" int mi_kv8_attention_f16(const void* q, int64_t q_stride, const void*
     a.layer = layer;
     a.num_blocks = num_blocks;
     a.window = static_cast<int>(std::min<int64_t>(window, int64_t{1} << 30));
-    a.c = scale * 1.4426950408889634f;
+    a.c = std::max(std::fabs(scale) * 1.4426950408889634f, 1e-37f);
+    a.neg = scale < 0.0f;
     a.count = static_cast<unsigned*>(workspace);
     a.part = static_cast<float*>(workspace) + kCounters;
+    Kv8Attn few, many;
+    int64_t need = 0;
+    const int pl = kv8_attn_plan(a, few, many, need);
+    if (pl != MI_OK) return pl;
+    if (need > 0 && (!workspace || workspace_bytes < need || !aligned16(workspace))) return MI_ERR_INVALID_ARGUMENT;
+    const void* bufs[6] = {k_cache, v_cache, k_scale, v_scale, q, workspace};
+    const int64_t lens[6] = {cells * block_size * head_dim, cells * block_size * head_dim, cells, cells, qb, need};
+    for (int i = 0; i < 6; ++i) {
+        if (overlaps(bufs[i], lens[i], out, ob)) return MI_ERR_ALIASING;
+        if (i < 5 && overlaps(bufs[i], lens[i], workspace, need)) return MI_ERR_ALIASING;
+    }
     const hipStream_t s = as_stream(stream);
-    const dim3 grid(static_cast<unsigned>(a.first[a.sg.n])), block(256);
-    if (head_dim <= 64) kv8_attn_kernel<64><<<grid, block, 0, s>>>(a);
-    else if (head_dim <= 128) kv8_attn_kernel<128><<<grid, block, 0, s>>>(a);
-    else kv8_attn_kernel<256><<<grid, block, 0, s>>>(a);
+    if (many.sg.n > 0) kv8_prompt_launch(many, s);
+    if (few.sg.n > 0) {
+        const dim3 grid(static_cast<unsigned>(few.first[few.sg.n])), block(256);
+        if (head_dim <= 64) kv8_attn_kernel<64><<<grid, block, 0, s>>>(few);
+        else if (head_dim <= 128) kv8_attn_kernel<128><<<grid, block, 0, s>>>(few);
+        else kv8_attn_kernel<256><<<grid, block, 0, s>>>(few);
+    }
     return launch_status();
 }
