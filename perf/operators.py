@@ -33,12 +33,18 @@ HEADS = ((28, 4, 128), (32, 8, 128), (14, 2, 64), (8, 4, 256), (16, 16, 64), (32
 MAX_START = 28000
 
 
+_library = None
+
+
 def _mk():
-    path = str(Path(__file__).resolve().parents[1] / "mini-infer_amd")
-    if path not in sys.path:
-        sys.path.insert(0, path)
-    import mi_kernels
-    return mi_kernels
+    global _library
+    if _library is None:
+        path = str(Path(__file__).resolve().parents[1] / "mini-infer_amd")
+        if path not in sys.path:
+            sys.path.insert(0, path)
+        import mi_kernels
+        _library = mi_kernels
+    return _library
 
 
 # --- the cases ---------------------------------------------------------------
