@@ -25,14 +25,17 @@ namespace mi {
 
 constexpr int kFewRows = 64;   // query rows of a (sequence, KV head) up to which tiles of 16 take them
 constexpr int kRows = 16;      // query rows of a tile: (token, head of the KV head's group)
-constexpr int kKeys = 64;      // keys of a wave's step
-constexpr int kWaves = 4;      // waves of a workgroup, each on every fourth step
-constexpr int64_t kWant = 2048;        // workgroups that a segment of few rows is split into
+constexpr int64_t kWant = 1024;        // workgroups that a segment of few rows is split into
 constexpr int64_t kPromptWant = 512;   // and one of many rows
-constexpr int64_t kCounters = kKv8Segs * kWant / 2;  // at the head of the workspace, zeros between calls
+constexpr int64_t kWide256 = 400;      // tiles of 256 rows from which on a call takes those, and not of 128
+constexpr int64_t kCounters = kKv8Segs * 1024;  // at the head of the workspace, zeros between calls
 
 template <int HD>
 struct Tile {
+    static constexpr int kWaves = 8;             // of a workgroup, each on every eighth step; two a SIMD
+    static constexpr int kLeast = 2 * kWaves;    // steps of a split, and what they are a multiple of
+    static constexpr int kKl = HD > 128 ? 8 : 16;  // keys of a step that a lane group has
+    static constexpr int kKeys = 4 * kKl;            // keys of a wave's step
     static constexpr int kSteps = HD / 32;   // MFMA steps of q . k
     static constexpr int kD = HD / 16;       // tiles of d; consecutive d of a lane in V
     static constexpr int kKw = HD / 16;      // dwords of K a lane holds per tile of 16 keys
@@ -41,7 +44,7 @@ struct Tile {
 
 // V's d column `j` of keys 8m .. 8m + 7 of the lane's block, as an MFMA operand.
 template <int HD>
-__device__ __forceinline__ void v_pair(const uint32_t (&raw)[16][Tile<HD>::kVw], int m, int word, int hi,
+__device__ __forceinline__ void v_pair(const uint32_t (&raw)[Tile<HD>::kKl][Tile<HD>::kVw], int m, int word, int hi,
                                        float scale, h8& even, h8& odd) {
     uint32_t e[4], o[4];
 #pragma unroll
@@ -70,8 +73,9 @@ __device__ __forceinline__ void v_pair(const uint32_t (&raw)[16][Tile<HD>::kVw],
 // read once the scores are made, V of the next after the sums, so a wave always has half a
 // step (8 KB at head_dim 128) in flight while it computes.
 template <int HD>
-__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn a) {
+__global__ __launch_bounds__(Tile<HD>::kWaves * 64, 2) void kv8_attn_kernel(Kv8Attn a) {
     using L = Tile<HD>;
+    constexpr int kWaves = L::kWaves, kThreads = kWaves * 64, KL = L::kKl, NT = KL / 4, kKeys = L::kKeys;
     __shared__ float s_ml[kWaves][2][kRows];
     __shared__ float s_o[kWaves][kRows][HD + 4];
     __shared__ bool s_last;
@@ -85,7 +89,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
     const int split = divmod(id, a.nsplit[g]);
     const int tile = divmod(id, a.tiles[g]);
     const int64_t b = id;
-    const TileKeys t = tile_keys<kRows, kKeys, kWaves>(a, g, b, tile);
+    const TileKeys t = tile_keys<kRows, kKeys, L::kLeast>(a, g, b, tile);
     if (split >= max(t.used, 1)) return;
     const int col = lane & 15, grp = lane >> 4;
     const int64_t tok0 = a.sg.off[g] + b * t.S;
@@ -124,15 +128,19 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
         return key < hi32 && static_cast<uint32_t>(phys) < static_cast<uint32_t>(nb) ? phys : -1;
     };
     const int64_t page0 = a.layer * a.num_blocks;
-    uint32_t kr[4][L::kKw], vr[16][L::kVw];
+    uint32_t kr[NT][L::kKw], vr[KL][L::kVw];
     int kbyte = 0, vbyte = 0, kphys = -1, vphys = -1, kin = 0, vin = 0, vnext = -1, vnin = 0;
-    const auto find_k = [&](int step) { kphys = page_of(step, col >> 2, kin); };
-    const auto find_v = [&](int step) { vnext = page_of(step, grp, vnin); };
+    // a lane group's keys of a step: all 16 of a block, or half of one
+    const int kgrp = col >> 2;  // the group whose keys this lane's row of K stands for
+    const auto blk_of = [](int group) { return KL == 16 ? group : group >> 1; };
+    const auto in_blk = [](int group) { return KL == 16 ? 0 : (group & 1) * 8; };
+    const auto find_k = [&](int step) { kphys = page_of(step, blk_of(kgrp), kin); };
+    const auto find_v = [&](int step) { vnext = page_of(step, blk_of(grp), vnin); };
     const auto load_k = [&] {
         const int64_t pg = (page0 + max(kphys, 0)) * a.Hkv + h;
-        const uint8_t* const p = a.kc + (pg * a.bs + kin + (col & 3)) * a.hd;
+        const uint8_t* const p = a.kc + (pg * a.bs + kin + in_blk(kgrp) + (col & 3)) * a.hd;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < NT; ++i)
 #pragma unroll
             for (int w = 0; w < L::kKw; w += 4) {
                 const int d = grp * (HD / 4) + w * 4;
@@ -144,9 +152,9 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
         vphys = vnext;
         vin = vnin;
         const int64_t pg = (page0 + max(vphys, 0)) * a.Hkv + h;
-        const uint8_t* const p = a.vc + (pg * a.bs + vin) * a.hd + (col * L::kD < a.hd ? col * L::kD : 0);
+        const uint8_t* const p = a.vc + (pg * a.bs + vin + in_blk(grp)) * a.hd + (col * L::kD < a.hd ? col * L::kD : 0);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) load_words<L::kVw>(vr[i], p + i * a.hd);
+        for (int i = 0; i < KL; ++i) load_words<L::kVw>(vr[i], p + i * a.hd);
         vbyte = a.vs[pg];
     };
 
@@ -170,9 +178,9 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
     for (; step < end; step += kWaves) {
         const float kscale = e8_scale(kbyte);
         // scores: tile i's row 4 g + e is key 4 i + e of block g
-        f4 sc[4];
+        f4 sc[NT];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < NT; ++i) {
             sc[i] = f4{0, 0, 0, 0};
 #pragma unroll
             for (int w = 0; w < L::kSteps; ++w) {
@@ -189,17 +197,17 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
         float vscale = e8_scale(vbyte);
         const int64_t key0 = t.base + static_cast<int64_t>(step) * kKeys;
         const bool masked = key0 + kKeys > all_hi || key0 < all_lo || key0 < t.lo || __any(vphys < 0);
-        uint32_t seen_by_any = 0, seen = 0xFFFF;  // of the lane's 16 keys, those that its row sees
+        uint32_t seen_by_any = 0, seen = 0xFFFF;  // of the lane's keys, those that its row sees
         bool nan_path = false;
-        float x[16];
+        float x[KL];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) x[i] = sc[i >> 2][i & 3] * a.c;
+        for (int i = 0; i < KL; ++i) x[i] = sc[i >> 2][i & 3] * a.c;
         if (masked) {
             seen = 0;
             uint32_t some = 0;  // and those that any row may see
-            const int64_t k0 = key0 + grp * 16;
+            const int64_t k0 = key0 + grp * KL;
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < KL; ++i) {
                 if (vphys >= 0 && k0 + i < row_hi && k0 + i >= row_lo) seen |= 1u << i;
                 if (vphys >= 0 && k0 + i < t.hi && k0 + i >= t.lo) some |= 1u << i;
                 if (!(seen & (1u << i))) x[i] = -INFINITY;
@@ -207,7 +215,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
             // what no row sees may hold anything, NaN too: 0 times it must be 0
             uint32_t nan = vphys >= 0 && vbyte == 255 ? some : 0;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < KL; ++i)
 #pragma unroll
                 for (int w = 0; w < L::kVw; ++w) {
                     if (!(some & (1u << i))) vr[i][w] = 0;
@@ -220,7 +228,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
         }
         float mx = x[0];
 #pragma unroll
-        for (int i = 1; i < 16; ++i) mx = fmaxf(mx, x[i]);
+        for (int i = 1; i < KL; ++i) mx = fmaxf(mx, x[i]);
         const float mn = fmaxf(m, max_over_groups(mx));
         if (__any(mn > m)) {
             const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
@@ -230,23 +238,23 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
             m = mn;
         }
         const float ref = (m == -INFINITY ? 0.0f : m) - kPShift;
-        h8 p[2];
+        h8 p[KL / 8];
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
+        for (int i = 0; i < KL; ++i) {
             const float w = __builtin_amdgcn_exp2f(x[i] - ref);
             l += w;
             p[i >> 3][i & 7] = (half_t)w;
         }
         if (nan_path) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < KL; ++i)
 #pragma unroll
                 for (int w = 0; w < L::kVw; ++w) vr[i][w] = vbyte == 255 ? 0u : vr[i][w] & ~nan_bytes(vr[i][w]);
         }
 #pragma unroll
         for (int j = 0; j < L::kD; j += 2)
 #pragma unroll
-            for (int k = 0; k < 2; ++k) {
+            for (int k = 0; k < KL / 8; ++k) {
                 h8 even, odd;
                 v_pair<HD>(vr, k, j >> 2, (j >> 1) & 1, vscale, even, odd);
                 o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p[k], o[j], 0, 0, 0);
@@ -254,15 +262,15 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
             }
         if (nan_path) {  // the rows that see one of the NaN: V again, as ones in their places
             const int64_t pg = (page0 + max(vphys, 0)) * a.Hkv + h;
-            const uint8_t* const q = a.vc + (pg * a.bs + vin) * a.hd + (col * L::kD < a.hd ? col * L::kD : 0);
-            h8 see[2];
+            const uint8_t* const q = a.vc + (pg * a.bs + vin + in_blk(grp)) * a.hd + (col * L::kD < a.hd ? col * L::kD : 0);
+            h8 see[KL / 8];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
+            for (int i = 0; i < KL; ++i) {
                 load_words<L::kVw>(vr[i], q + i * a.hd);
                 see[i >> 3][i & 7] = (half_t)(seen & (1u << i) ? 1.0f : 0.0f);
             }
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
+            for (int i = 0; i < KL; ++i)
 #pragma unroll
                 for (int w = 0; w < L::kVw; ++w)  // 0x38: one
                     vr[i][w] = seen_by_any & (1u << i) ? 0x38383838u & (vbyte == 255 ? ~0u : nan_bytes(vr[i][w])) : 0u;
@@ -270,7 +278,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
             for (int j = 0; j < L::kD; j += 2) {
                 f4 n0 = f4{0, 0, 0, 0}, n1 = n0;
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
+                for (int k = 0; k < KL / 8; ++k) {
                     h8 even, odd;
                     v_pair<HD>(vr, k, j >> 2, (j >> 1) & 1, 1.0f, even, odd);
                     n0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, see[k], n0, 0, 0, 0);
@@ -309,7 +317,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
         const bool rl = rp >= 0 && rp < t.sl && tot != 0.0f;
         a.out[(tok0 + rs) * a.os + (h * a.G + rr - rs * a.G) * a.hd + d] = (half_t)(rl ? sum / tot : 0.0f);
     };
-    for (int i = threadIdx.x; i < t.rows * a.hd; i += 256) {
+    for (int i = threadIdx.x; i < t.rows * a.hd; i += kThreads) {
         const int r = small_div(i, inv_hd), d = i - r * a.hd;
         float mm = -INFINITY;
 #pragma unroll
@@ -346,13 +354,20 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
     if (!s_last) return;
     if (threadIdx.x == 0) *counter = 0;  // for the next call
     float* const w_of = &s_o[0][0][0];   // [split][row], then the rows' sums
-    static_assert(kMaxSplits * kRows * 2 + kRows <= kWaves * kRows * (64 + 4), "the splits' weights fit");
+    static_assert(kMaxSplits * kRows * 2 <= kWaves * kRows * (HD + 4), "the splits' weights fit");
     float* const l_of = w_of + kMaxSplits * kRows;
-    for (int i = threadIdx.x; i < t.used * t.rows; i += 256) {
+    for (int i = threadIdx.x; i < t.used * t.rows; i += kThreads) {
         const int sp = i / t.rows, r = i - sp * t.rows;
         w_of[sp * kRows + r] = load_agent(part + sp * apart + r * (a.hd + 2) + a.hd);
         l_of[sp * kRows + r] = load_agent(part + sp * apart + r * (a.hd + 2) + a.hd + 1);
     }
+    // the first splits' sums are asked for before their weights are known
+    constexpr int kAhead = 8;
+    float ahead[kAhead];
+    const int r0 = small_div(threadIdx.x, inv_hd), d0 = threadIdx.x - r0 * a.hd;
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+        ahead[k] = load_agent(part + min(k, t.used - 1) * apart + (r0 < t.rows ? r0 * (a.hd + 2) + d0 : 0));
     __syncthreads();
     if (threadIdx.x < t.rows) {
         const int r = threadIdx.x;
@@ -367,11 +382,17 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
         s_ml[0][0][r] = tot;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < t.rows * a.hd; i += 256) {
+    for (int i = threadIdx.x; i < t.rows * a.hd; i += kThreads) {
         const int r = small_div(i, inv_hd), d = i - r * a.hd;
         const float* const p = part + r * (a.hd + 2) + d;
         float sum = 0.0f;
         int sp = 0;
+        if (i == static_cast<int>(threadIdx.x)) {
+#pragma unroll
+            for (int k = 0; k < kAhead; ++k)
+                if (k < t.used) sum = fmaf(ahead[k], w_of[k * kRows + r], sum);
+            sp = min(kAhead, t.used);
+        }
         for (; sp + 8 <= t.used; sp += 8) {
             float v[8];
 #pragma unroll
@@ -390,7 +411,11 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_attn_kernel(Kv8Attn
 static int kv8_attn_plan(const Kv8Attn& all, Kv8Attn& few, Kv8Attn& many, int64_t& bytes) {
     few = many = all;
     few.sg.n = many.sg.n = 0;
-    int64_t floats = 0, counters = 0;
+    few.rows = kRows;
+    int64_t floats = 0, counters = 0, wide256 = 0;
+    for (int i = 0; i < all.sg.n; ++i)
+        if (all.sg.S[i] * all.G > kFewRows) wide256 += all.sg.B[i] * ceil_div(all.sg.S[i] * all.G, 256) * all.Hkv;
+    many.rows = wide256 >= kWide256 ? 256 : 128;
     for (int i = 0; i < all.sg.n; ++i) {
         const int64_t rows = all.sg.S[i] * all.G;
         const bool wide = rows > kFewRows;
@@ -403,7 +428,7 @@ static int kv8_attn_plan(const Kv8Attn& all, Kv8Attn& few, Kv8Attn& many, int64_
         a.sg.bt[n] = all.sg.bt[i];
         a.sg.sl[n] = all.sg.sl[i];
         a.sg.sp[n] = all.sg.sp[i];
-        const int64_t tile = wide ? kPromptRows : kRows, tiles = ceil_div(rows, tile);
+        const int64_t tile = a.rows, tiles = ceil_div(rows, tile);
         const int64_t groups = a.sg.B[n] * tiles * a.Hkv;
         const int64_t ns = std::clamp<int64_t>((wide ? kPromptWant : kWant) / std::max<int64_t>(groups, 1), 1,
                                                std::min<int64_t>(a.sg.mb[n], kMaxSplits));
@@ -520,10 +545,10 @@ extern "C" int mi_kv8_attention_f16(const void* q, int64_t q_stride, const void*
     const hipStream_t s = as_stream(stream);
     if (many.sg.n > 0) kv8_prompt_launch(many, s);
     if (few.sg.n > 0) {
-        const dim3 grid(static_cast<unsigned>(few.first[few.sg.n])), block(256);
-        if (head_dim <= 64) kv8_attn_kernel<64><<<grid, block, 0, s>>>(few);
-        else if (head_dim <= 128) kv8_attn_kernel<128><<<grid, block, 0, s>>>(few);
-        else kv8_attn_kernel<256><<<grid, block, 0, s>>>(few);
+        const dim3 grid(static_cast<unsigned>(few.first[few.sg.n]));
+        if (head_dim <= 64) kv8_attn_kernel<64><<<grid, dim3(Tile<64>::kWaves * 64), 0, s>>>(few);
+        else if (head_dim <= 128) kv8_attn_kernel<128><<<grid, dim3(Tile<128>::kWaves * 64), 0, s>>>(few);
+        else kv8_attn_kernel<256><<<grid, dim3(Tile<256>::kWaves * 64), 0, s>>>(few);
     }
     return launch_status();
 }

@@ -9,6 +9,7 @@ namespace mi {
 typedef float f4 __attribute__((ext_vector_type(4)));
 
 constexpr float kPShift = 14.0f;  // the softmax's weights are rounded to fp16 times 2^14
+constexpr float kSlack = 1.5f;   // how far a maximum may rise before the sums are scaled again
 constexpr int kMaxSplits = 64;
 
 struct Kv8Attn {
@@ -17,6 +18,7 @@ struct Kv8Attn {
     const uint8_t *kc, *vc, *ks, *vs;
     int64_t qs, os, num_blocks, layer;
     int Hq, Hkv, G, hd, bs, window;
+    int rows;  // query rows of a tile
     float c;   // |scale| * log2(e), above 0: a hidden score times it stays -inf
     bool neg;  // scale < 0: q is negated
     float* part;      // the workspace: partial sums of the splits
@@ -106,8 +108,7 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
     return top | (top - (top >> 7));
 }
 
-// Segments of many query rows (kv8_prompt.hip), already planned.
+// Segments of many query rows (kv8_prompt.hip), planned in tiles of 128 or 256.
 void kv8_prompt_launch(const Kv8Attn& a, hipStream_t s);
-constexpr int kPromptRows = 128;  // query rows of its tile
 
 }  // namespace mi

@@ -28,9 +28,19 @@ __device__ __forceinline__ int v_piece(int d, int c) {
     else return c ^ (((d >> 2) & 3) ^ (d & 2));
 }
 
-template <int HD>
-__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8Attn a) {
+// The next `n` instructions of a kind, in the scheduler's order.
+constexpr int kMfma = 0x8, kDsRead = 0x100;
+template <int KIND>
+__device__ __forceinline__ void order(int n) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) __builtin_amdgcn_sched_group_barrier(KIND, 1, 0);
+}
+
+template <int HD, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, HD > 128 ? WAVES / 4 : 2) void kv8_prompt_kernel(Kv8Attn a) {
     constexpr int KT = prompt_keys<HD>();
+    constexpr int kRowsT = WAVES * 32;        // query rows
+    constexpr bool kRoles = WAVES == 8;       // the first four waves bring K, the others V
     constexpr int kSub = KT / 32;             // 32-key subtiles
     constexpr int kSteps = HD / 16;           // MFMA steps of q . k
     constexpr int kDt = HD / 32;              // 32-wide tiles of d
@@ -53,7 +63,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     // a sequence's last tiles have the most keys: first
     const int64_t b = id % static_cast<uint32_t>(a.sg.B[g]);
     const int tile = a.tiles[g] - 1 - static_cast<int>(id / static_cast<uint32_t>(a.sg.B[g]));
-    const TileKeys t = tile_keys<kPromptRows, KT, 4>(a, g, b, tile);
+    const TileKeys t = tile_keys<kRowsT, KT, 4>(a, g, b, tile);
     if (split >= max(t.used, 1)) return;
     const int64_t tok0 = a.sg.off[g] + b * t.S;
 
@@ -97,68 +107,92 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     };
 
     // what this lane brings of a tile: of K, units of 16 bytes of a key; of V, four d of eight keys
-    const int vk = tid / (HD / 4) * 8, vd = tid % (HD / 4) * 4;
-    const bool has_v = kAllV || vk < KT;
+    const int lid = kRoles ? tid & 255 : tid;
+    const bool has_k = !kRoles || wave < 4;
+    const int vk = lid / (HD / 4) * 8, vd = lid % (HD / 4) * 4;
+    const bool has_v = (!kRoles || wave >= 4) && (kAllV || vk < KT);
+    const uint32_t page_bytes = static_cast<uint32_t>(a.Hkv * a.bs * a.hd);  // of all heads: < 2^31
+    const uint8_t* const kbase = a.kc + (page0 * a.Hkv + h) * a.bs * a.hd;
+    const uint8_t* const vbase = a.vc + (page0 * a.Hkv + h) * a.bs * a.hd + (vk & 8) * a.hd + (vd < a.hd ? vd : 0);
+    const uint8_t *const ksc = a.ks + page0 * a.Hkv + h, *const vsc = a.vs + page0 * a.Hkv + h;
+    int koff[kKu];
+#pragma unroll
+    for (int u = 0; u < kKu; ++u) {
+        const int key = (lid + u * 256) / (HD / 16) & 15, d = (lid + u * 256) % (HD / 16) * 16;
+        koff[u] = key * a.hd + (d < a.hd ? d : 0);
+    }
     uint32_t kraw[kKu][4], vraw[8];
     int kb[kKu], vb = 0, vphys = -1, vfound = -1, vin = 0, kphys[kKu], kin[kKu];
     const auto find = [&](int step) {
         const int key0 = base32 + step * KT;
+        if (has_k) {
 #pragma unroll
-        for (int u = 0; u < kKu; ++u) kphys[u] = page_of(key0 + ((tid + u * 256) / (HD / 16) & ~15), kin[u]);
-        vfound = page_of(key0 + ((has_v ? vk : 0) & ~15), vin);
+            for (int u = 0; u < kKu; ++u) kphys[u] = page_of(key0 + ((lid + u * 256) / (HD / 16) & ~15), kin[u]);
+        }
+        // every lane, as it also says which blocks of the tile have a page
+        vfound = page_of(key0 + ((kAllV || vk < KT ? vk : 0) & ~15), vin);
     };
     const auto load = [&] {
-#pragma unroll
-        for (int u = 0; u < kKu; ++u) {
-            const int key = (tid + u * 256) / (HD / 16) & 15, d = (tid + u * 256) % (HD / 16) * 16;
-            const int64_t pg = (page0 + max(kphys[u], 0)) * a.Hkv + h;
-            load_words<4>(kraw[u], a.kc + (pg * a.bs + kin[u] + key) * a.hd + (d < a.hd ? d : 0));
-            kb[u] = a.ks[pg];
-        }
         vphys = vfound;
-        const int64_t pg = (page0 + max(vphys, 0)) * a.Hkv + h;
-        const uint8_t* const p = a.vc + (pg * a.bs + vin + (vk & 8)) * a.hd + (vd < a.hd ? vd : 0);
+        if (has_k) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) load_words<1>(&vraw[i], p + i * a.hd);
-        vb = a.vs[pg];
-    };
-    const auto store = [&](int step, int buf) {
-#pragma unroll
-        for (int u = 0; u < kKu; ++u) {
-            const int key = (tid + u * 256) / (HD / 16), c = (tid + u * 256) % (HD / 16) * 2;
-            const float scale = e8_scale(kb[u]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const h2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i], scale, false);
-                const h2 x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i], scale, true);
-                const h2 x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i + 1], scale, false);
-                const h2 x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i + 1], scale, true);
-                *reinterpret_cast<h8*>(&s_k[buf][key * HD + k_piece(key, c + i) * 8]) =
-                    h8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+            for (int u = 0; u < kKu; ++u) {
+                const uint32_t pg = max(kphys[u], 0);
+                load_words<4>(kraw[u], kbase + static_cast<uint64_t>(pg) * page_bytes + (kin[u] * a.hd + koff[u]));
+                kb[u] = ksc[static_cast<uint64_t>(pg) * static_cast<uint32_t>(a.Hkv)];
             }
         }
-        // V: what no row may see is zero, whatever it holds
-        const int key0 = base32 + step * KT + vk;
-        // and NaN is zero with its place kept in s_bits
-        const bool ok = vphys >= 0 && key0 < hi32 && key0 + 8 > lo32;
-        const bool all_nan = ok && vb == 255;
-        const float scale = e8_scale(ok && !all_nan ? vb : kE8Bias);
-        uint32_t nan = all_nan ? 1u : 0u, bits = 0;
+        if (!kRoles || wave >= 4) {
+            const uint32_t pg = max(vphys, 0);
+            const uint8_t* p = vbase + static_cast<uint64_t>(pg) * page_bytes + vin * a.hd;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (!ok || key0 + i >= hi32 || key0 + i < lo32) vraw[i] = 0;
-            nan |= nan_bytes(vraw[i]);
+            for (int i = 0; i < 8; ++i, p += a.hd) load_words<1>(&vraw[i], p);
+            vb = vsc[static_cast<uint64_t>(pg) * static_cast<uint32_t>(a.Hkv)];
         }
-        if (nan) {
+    };
+    const auto store = [&](int step, int buf) {
+        if (has_k) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bool in = key0 + i < hi32 && key0 + i >= lo32;
-                const uint32_t n = all_nan ? (in ? ~0u : 0u) : nan_bytes(vraw[i]);
-                bits |= (n & 0x01010101u) << i;
-                vraw[i] &= ~n;
+            for (int u = 0; u < kKu; ++u) {
+                const int key = (lid + u * 256) / (HD / 16), c = (lid + u * 256) % (HD / 16) * 2;
+                const float scale = e8_scale(kb[u]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const h2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i], scale, false);
+                    const h2 x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i], scale, true);
+                    const h2 x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i + 1], scale, false);
+                    const h2 x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i + 1], scale, true);
+                    *reinterpret_cast<h8*>(&s_k[buf][key * HD + k_piece(key, c + i) * 8]) =
+                        h8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+                }
             }
         }
         if (has_v) {
+            // what no row may see is zero, whatever it holds, and NaN is zero with its place
+            // kept in s_bits
+            const int tile0 = base32 + step * KT, key0 = tile0 + vk;
+            float scale = e8_scale(vb);
+            uint32_t nan = vb == 255 ? 0x80u : 0u, bits = 0;
+            if (tile0 + KT > hi32 || tile0 < lo32 || __any(vphys < 0)) {
+                const bool ok = vphys >= 0 && key0 < hi32 && key0 + 8 > lo32;
+                if (!ok) scale = 1.0f, nan = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (!ok || key0 + i >= hi32 || key0 + i < lo32) vraw[i] = 0;
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) nan |= (vraw[i] & 0x7F7F7F7Fu) + 0x01010101u;
+            if (nan & 0x80808080u) {
+                const bool all_nan = __builtin_bit_cast(uint32_t, scale) >> 23 == 255;
+                if (all_nan) scale = 1.0f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const bool in = key0 + i < hi32 && key0 + i >= lo32;
+                    const uint32_t n = all_nan ? (in ? ~0u : 0u) : nan_bytes(vraw[i]);
+                    bits |= (n & 0x01010101u) << i;
+                    vraw[i] &= ~n;
+                }
+            }
             uint32_t w[4][4];  // [d][pair of keys]
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -203,21 +237,41 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
         const int key0 = base32 + step * KT;
         const half_t *const sk = s_k[buf], *const sv = s_v[buf];
         if (some_row && key0 < any_hi && key0 + KT > any_lo) {
+            // Each fragment is asked for while the products before it run: LDS answers in some
+            // 100 cycles, a product takes 32.
             f16v sc[kSub];
-#pragma unroll
-            for (int ks = 0; ks < kSub; ++ks) {
-                sc[ks] = f16v(0);
+            h8 kf[2][kSteps], vf[2][kSub * 2];
+            const auto k_read = [&](int ks) {
                 // row 16 i + 8 j + 4 f + e of the subtile stands for key 16 i + 8 f + 4 j + e
                 const int key = ks * 32 + (col & 0x13) + ((col & 4) << 1) + ((col & 8) >> 1);
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    const h8 kf = ld8(sk + key * HD + k_piece(key, 2 * i + hf) * 8);
-                    sc[ks] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[i], sc[ks], 0, 0, 0);
-                }
-            }
-            bool masked = key0 + KT > all_hi || key0 < all_lo;
+                for (int i = 0; i < kSteps; ++i) kf[ks & 1][i] = ld8(sk + key * HD + k_piece(key, 2 * i + hf) * 8);
+            };
+            const auto v_read = [&](int j) {
+                const int d = j * 32 + col;
 #pragma unroll
-            for (int i = 0; i < KT / 16; ++i) masked |= s_ok[buf][i] == 0;
+                for (int k = 0; k < kSub * 2; ++k) vf[j & 1][k] = ld8(sv + d * KT + v_piece<KT>(d, 2 * k + hf) * 8);
+            };
+            k_read(0);
+#pragma unroll
+            for (int ks = 0; ks < kSub; ++ks) {
+                if (ks + 1 < kSub) k_read(ks + 1);
+                else v_read(0);
+                sc[ks] = f16v(0);
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i)
+                    sc[ks] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[ks & 1][i], qf[i], sc[ks], 0, 0, 0);
+            }
+            order<kDsRead>(kSteps);
+#pragma unroll
+            for (int i = 0; i < kSub * kSteps; ++i) {
+                order<kMfma>(1);
+                order<kDsRead>(1);
+            }
+            int in_cache = 1;
+#pragma unroll
+            for (int i = 0; i < KT / 16; ++i) in_cache &= s_ok[buf][i];
+            const bool masked = key0 + KT > all_hi || key0 < all_lo || __builtin_amdgcn_readfirstlane(in_cache) == 0;
             if (masked) {
 #pragma unroll
                 for (int ks = 0; ks < kSub; ++ks)
@@ -236,7 +290,8 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
             pair_xor32(__builtin_bit_cast(uint32_t, mx), pa, pb);
             mx = fmaxf(__builtin_bit_cast(float, pa), __builtin_bit_cast(float, pb));
             const float mn = fmaxf(m, mx * a.c);  // a.c > 0
-            if (__any(mn > m)) {
+            // the reference follows the maximum only where the weights would grow past 2^15.5
+            if (__any(mn > m + kSlack)) {
                 const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
                 l *= by;
 #pragma unroll
@@ -255,14 +310,17 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
                 }
 #pragma unroll
             for (int j = 0; j < kDt; ++j) {
-                const int d = j * 32 + col;
+                if (j + 1 < kDt) v_read(j + 1);
 #pragma unroll
-                for (int k = 0; k < kSub * 2; ++k) {
-                    const h8 vf = ld8(sv + d * KT + v_piece<KT>(d, 2 * k + hf) * 8);
-                    o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf, p[k], o[j], 0, 0, 0);
-                }
+                for (int k = 0; k < kSub * 2; ++k)
+                    o[j] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[j & 1][k], p[k], o[j], 0, 0, 0);
             }
-            if (s_nan[buf] == step) {  // rare: a NaN reaches the rows that see its key, and no other
+#pragma unroll
+            for (int i = 0; i < kDt * kSub * 2; ++i) {
+                order<kMfma>(1);
+                order<kDsRead>(1);
+            }
+            if (__builtin_amdgcn_readfirstlane(s_nan[buf]) == step) {  // rare: a NaN reaches the rows that see its key, and no other
                 uint8_t see[KT / 8];
 #pragma unroll
                 for (int c = 0; c < KT / 8; ++c) {
@@ -312,7 +370,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     }
     // partial sums [split][d, maximum, sum][row]
     const int64_t group = (b * a.tiles[g] + tile) * a.Hkv + h;
-    const int64_t apart = static_cast<int64_t>(kPromptRows) * (a.hd + 2);
+    const int64_t apart = static_cast<int64_t>(kRowsT) * (a.hd + 2);
     float* const part = a.part + a.part0[g] + group * a.nsplit[g] * apart;
     {
         float* const to = part + split * apart + wave * 32 + col;
@@ -321,11 +379,11 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const int d = j * 32 + (i >> 2) * 8 + hf * 4 + (i & 3);
-                if (d < a.hd) store_agent(to + d * kPromptRows, o[j][i]);
+                if (d < a.hd) store_agent(to + d * kRowsT, o[j][i]);
             }
         if (hf == 0) {
-            store_agent(to + a.hd * kPromptRows, m);
-            store_agent(to + (a.hd + 1) * kPromptRows, l);
+            store_agent(to + a.hd * kRowsT, m);
+            store_agent(to + (a.hd + 1) * kRowsT, l);
         }
     }
     __builtin_amdgcn_s_waitcnt(kDrainVmem);
@@ -337,27 +395,27 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     __syncthreads();
     if (!s_last) return;
     if (tid == 0) *counter = 0;
-    const int r = tid & (kPromptRows - 1);
+    const int r = tid & (kRowsT - 1);
     if (r >= t.rows) return;
     const float* const from = part + r;
     float mm = -INFINITY, tot = 0.0f;
-    for (int sp = 0; sp < t.used; ++sp) mm = fmaxf(mm, load_agent(from + sp * apart + a.hd * kPromptRows));
+    for (int sp = 0; sp < t.used; ++sp) mm = fmaxf(mm, load_agent(from + sp * apart + a.hd * kRowsT));
     const float ref = mm == -INFINITY ? 0.0f : mm;
     const auto weight = [&](int sp) {
-        return join_weight(load_agent(from + sp * apart + a.hd * kPromptRows),
-                           load_agent(from + sp * apart + (a.hd + 1) * kPromptRows), ref);
+        return join_weight(load_agent(from + sp * apart + a.hd * kRowsT),
+                           load_agent(from + sp * apart + (a.hd + 1) * kRowsT), ref);
     };
     for (int sp = 0; sp < t.used; ++sp)
-        tot = fmaf(load_agent(from + sp * apart + (a.hd + 1) * kPromptRows), weight(sp), tot);
+        tot = fmaf(load_agent(from + sp * apart + (a.hd + 1) * kRowsT), weight(sp), tot);
     const auto [to, on] = out_row(r);
     const bool some = on && tot != 0.0f;
-    for (int d = tid / kPromptRows * 8; d < a.hd; d += 16) {
+    for (int d = tid / kRowsT * 8; d < a.hd; d += 16) {  // two lanes per row
         float sum[8] = {};
         for (int sp = 0; sp < t.used; ++sp) {
             const float w = weight(sp);
             float v[8];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = load_agent(from + sp * apart + (d + e) * kPromptRows);
+            for (int e = 0; e < 8; ++e) v[e] = load_agent(from + sp * apart + (d + e) * kRowsT);
 #pragma unroll
             for (int e = 0; e < 8; ++e) sum[e] = fmaf(v[e], w, sum[e]);
         }
@@ -366,11 +424,17 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     }
 }
 
+template <int WAVES>
+static void prompt_go(const Kv8Attn& a, hipStream_t s) {
+    const dim3 grid(static_cast<unsigned>(a.first[a.sg.n])), block(WAVES * 64);
+    if (a.hd <= 64) kv8_prompt_kernel<64, WAVES><<<grid, block, 0, s>>>(a);
+    else if (a.hd <= 128) kv8_prompt_kernel<128, WAVES><<<grid, block, 0, s>>>(a);
+    else kv8_prompt_kernel<256, WAVES><<<grid, block, 0, s>>>(a);
+}
+
 void kv8_prompt_launch(const Kv8Attn& a, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(a.first[a.sg.n])), block(256);
-    if (a.hd <= 64) kv8_prompt_kernel<64><<<grid, block, 0, s>>>(a);
-    else if (a.hd <= 128) kv8_prompt_kernel<128><<<grid, block, 0, s>>>(a);
-    else kv8_prompt_kernel<256><<<grid, block, 0, s>>>(a);
+    if (a.rows == 256) prompt_go<8>(a, s);
+    else prompt_go<4>(a, s);
 }
 
 }  // namespace mi
