@@ -27,7 +27,6 @@ constexpr int kFewRows = 64;   // query rows of a (sequence, KV head) up to whic
 constexpr int kRows = 16;      // query rows of a tile: (token, head of the KV head's group)
 constexpr int64_t kWant = 1024;        // workgroups that a segment of few rows is split into
 constexpr int64_t kPromptWant = 512;   // and one of many rows
-constexpr int64_t kWide256 = 400;      // tiles of 256 rows from which on a call takes those, and not of 128
 constexpr int64_t kCounters = kKv8Segs * 1024;  // at the head of the workspace, zeros between calls
 
 template <int HD>
@@ -411,11 +410,7 @@ __global__ __launch_bounds__(Tile<HD>::kWaves * 64, 2) void kv8_attn_kernel(Kv8A
 static int kv8_attn_plan(const Kv8Attn& all, Kv8Attn& few, Kv8Attn& many, int64_t& bytes) {
     few = many = all;
     few.sg.n = many.sg.n = 0;
-    few.rows = kRows;
-    int64_t floats = 0, counters = 0, wide256 = 0;
-    for (int i = 0; i < all.sg.n; ++i)
-        if (all.sg.S[i] * all.G > kFewRows) wide256 += all.sg.B[i] * ceil_div(all.sg.S[i] * all.G, 256) * all.Hkv;
-    many.rows = wide256 >= kWide256 ? 256 : 128;
+    int64_t floats = 0, counters = 0;
     for (int i = 0; i < all.sg.n; ++i) {
         const int64_t rows = all.sg.S[i] * all.G;
         const bool wide = rows > kFewRows;
@@ -428,10 +423,10 @@ static int kv8_attn_plan(const Kv8Attn& all, Kv8Attn& few, Kv8Attn& many, int64_
         a.sg.bt[n] = all.sg.bt[i];
         a.sg.sl[n] = all.sg.sl[i];
         a.sg.sp[n] = all.sg.sp[i];
-        const int64_t tile = a.rows, tiles = ceil_div(rows, tile);
+        const int64_t tile = wide ? kPromptRows : kRows, tiles = ceil_div(rows, tile);
         const int64_t groups = a.sg.B[n] * tiles * a.Hkv;
         const int64_t ns = std::clamp<int64_t>((wide ? kPromptWant : kWant) / std::max<int64_t>(groups, 1), 1,
-                                               std::min<int64_t>(a.sg.mb[n], kMaxSplits));
+                                               std::min<int64_t>(a.sg.mb[n], wide ? kPromptSplits : kMaxSplits));
         a.tiles[n] = static_cast<int>(tiles);
         a.nsplit[n] = static_cast<int>(ns);
         a.first[n + 1] = a.first[n] + groups * ns;

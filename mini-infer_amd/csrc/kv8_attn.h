@@ -18,7 +18,6 @@ struct Kv8Attn {
     const uint8_t *kc, *vc, *ks, *vs;
     int64_t qs, os, num_blocks, layer;
     int Hq, Hkv, G, hd, bs, window;
-    int rows;  // query rows of a tile
     float c;   // |scale| * log2(e), above 0: a hidden score times it stays -inf
     bool neg;  // scale < 0: q is negated
     float* part;      // the workspace: partial sums of the splits
@@ -108,7 +107,9 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
     return top | (top - (top >> 7));
 }
 
-// Segments of many query rows (kv8_prompt.hip), planned in tiles of 128 or 256.
+// Segments of many query rows (kv8_prompt.hip), already planned.
 void kv8_prompt_launch(const Kv8Attn& a, hipStream_t s);
+constexpr int kPromptRows = 128;   // query rows of its tile
+constexpr int kPromptSplits = 32;  // at most
 
 }  // namespace mi

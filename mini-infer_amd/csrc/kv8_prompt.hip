@@ -14,6 +14,7 @@ namespace mi {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
+typedef const __attribute__((address_space(4))) int uniform_int;  // read through the scalar cache
 
 // Keys of a tile: what two LDS buffers of K and V and two workgroups per CU allow.
 template <int HD>
@@ -36,18 +37,19 @@ __device__ __forceinline__ void order(int n) {
     for (int i = 0; i < n; ++i) __builtin_amdgcn_sched_group_barrier(KIND, 1, 0);
 }
 
-template <int HD, int WAVES>
-__global__ __launch_bounds__(WAVES * 64, HD > 128 ? WAVES / 4 : 2) void kv8_prompt_kernel(Kv8Attn a) {
+template <int HD>
+__global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8Attn a) {
     constexpr int KT = prompt_keys<HD>();
-    constexpr int kRowsT = WAVES * 32;        // query rows
-    constexpr bool kRoles = WAVES == 8;       // the first four waves bring K, the others V
     constexpr int kSub = KT / 32;             // 32-key subtiles
     constexpr int kSteps = HD / 16;           // MFMA steps of q . k
     constexpr int kDt = HD / 32;              // 32-wide tiles of d
     constexpr int kKu = KT * HD / 16 / 256;   // 16-byte units of K a lane converts
     constexpr bool kAllV = KT / 8 * (HD / 4) >= 256;
-    __shared__ __attribute__((aligned(16))) half_t s_k[2][KT * HD];
-    __shared__ __attribute__((aligned(16))) half_t s_v[2][KT * HD];
+    constexpr int kTileBytes = KT * HD * 2;
+    // two tiles of K and of V; afterwards the rows of the output
+    __shared__ __attribute__((aligned(16))) uint8_t s_mem[4 * kTileBytes];
+    const auto s_k = reinterpret_cast<half_t(*)[KT * HD]>(s_mem);
+    const auto s_v = reinterpret_cast<half_t(*)[KT * HD]>(s_mem + 2 * kTileBytes);
     __shared__ int s_ok[2][KT / 16], s_nan[2];
     __shared__ __attribute__((aligned(4))) uint8_t s_bits[2][KT / 8][HD];  // V's NaN: a bit per key
     __shared__ bool s_last;
@@ -63,7 +65,7 @@ __global__ __launch_bounds__(WAVES * 64, HD > 128 ? WAVES / 4 : 2) void kv8_prom
     // a sequence's last tiles have the most keys: first
     const int64_t b = id % static_cast<uint32_t>(a.sg.B[g]);
     const int tile = a.tiles[g] - 1 - static_cast<int>(id / static_cast<uint32_t>(a.sg.B[g]));
-    const TileKeys t = tile_keys<kRowsT, KT, 4>(a, g, b, tile);
+    const TileKeys t = tile_keys<kPromptRows, KT, 4>(a, g, b, tile);
     if (split >= max(t.used, 1)) return;
     const int64_t tok0 = a.sg.off[g] + b * t.S;
 
@@ -71,7 +73,7 @@ __global__ __launch_bounds__(WAVES * 64, HD > 128 ? WAVES / 4 : 2) void kv8_prom
     const int w0 = t.r0 + wave * 32;  // the wave's first row
     const int row = w0 + col, s = row / a.G, head = h * a.G + (row - s * a.G);
     const int64_t pos = t.sp + s;
-    const bool mine = wave * 32 + col < t.rows, live = mine && pos >= 0 && pos < t.sl;
+    const bool live = wave * 32 + col < t.rows && pos >= 0 && pos < t.sl;
     const int row_hi = live ? static_cast<int>(min(pos + 1, t.hi)) : 0;
     const int row_lo = a.window > 0 ? static_cast<int>(min<int64_t>(max<int64_t>(pos - a.window + 1, 0), INT32_MAX)) : 0;
     h8 qf[kSteps];
@@ -92,107 +94,103 @@ __global__ __launch_bounds__(WAVES * 64, HD > 128 ? WAVES / 4 : 2) void kv8_prom
 
     const int* const table = a.sg.bt[g] + b * a.sg.mb[g];
     const int sub = a.bs >> 4;
-    const float inv_sub = 1.0f / static_cast<float>(sub);
     const int nb = static_cast<int>(a.num_blocks);
     const int end = min((split + 1) * t.per, t.steps);
     const int base32 = static_cast<int>(t.base), lo32 = static_cast<int>(t.lo);
     const int hi32 = min(static_cast<int>(t.hi), base32 + end * KT);
     const int64_t page0 = a.layer * a.num_blocks;
-    const auto page_of = [&](int key, int& in_page) {  // as in kv8_attention.hip: every load is made
-        const int k16 = key >> 4;
-        const int idx = small_div(k16, inv_sub);
-        in_page = (k16 - idx * sub) * 16;
-        const int phys = table[key < hi32 ? idx : 0];
+    const uint64_t inv_sub = ((uint64_t{1} << 40) + sub - 1) / static_cast<uint32_t>(sub);
+    const auto page_of = [&](int key, int& in_page) {  // of a 16-key block, -1 where it has none
+        const uint32_t k16 = static_cast<uint32_t>(key) >> 4;  // < 2^22, sub <= 256: the quotient is exact
+        const uint32_t idx = static_cast<uint32_t>(k16 * inv_sub >> 40);
+        in_page = static_cast<int>(k16 - idx * sub) * 16;
+        const int phys = reinterpret_cast<uniform_int*>(reinterpret_cast<uintptr_t>(table))[key < hi32 ? idx : 0];
         return key < hi32 && static_cast<uint32_t>(phys) < static_cast<uint32_t>(nb) ? phys : -1;
     };
 
-    // what this lane brings of a tile: of K, units of 16 bytes of a key; of V, four d of eight keys
-    const int lid = kRoles ? tid & 255 : tid;
-    const bool has_k = !kRoles || wave < 4;
-    const int vk = lid / (HD / 4) * 8, vd = lid % (HD / 4) * 4;
-    const bool has_v = (!kRoles || wave >= 4) && (kAllV || vk < KT);
-    const uint32_t page_bytes = static_cast<uint32_t>(a.Hkv * a.bs * a.hd);  // of all heads: < 2^31
+    // What a wave brings of a tile: units of 16 bytes of a key of K, four d of eight keys of V.  Its
+    // keys of a unit lie in one 16-key block, so that the block's page, scale and place are found by
+    // the scalar unit, and a lane adds an offset that never changes.
+    const int vk = kAllV ? tid / (HD / 4) * 8 : wave * 16 + (lane >> 4 & 1) * 8, vd = tid % (HD / 4) * 4;
+    const bool has_v = kAllV || lane < 32;  // (heads of 64: half of a wave brings a block of V)
+    const auto k_block = [&](int u) { return (wave * 64 + u * 256) / (HD / 16) >> 4; };
+    const int v_block = kAllV ? wave * 64 / (HD / 4) * 8 >> 4 : wave;
+    const int64_t page_bytes = static_cast<int64_t>(a.Hkv) * a.bs * a.hd;
     const uint8_t* const kbase = a.kc + (page0 * a.Hkv + h) * a.bs * a.hd;
-    const uint8_t* const vbase = a.vc + (page0 * a.Hkv + h) * a.bs * a.hd + (vk & 8) * a.hd + (vd < a.hd ? vd : 0);
-    const uint8_t *const ksc = a.ks + page0 * a.Hkv + h, *const vsc = a.vs + page0 * a.Hkv + h;
-    int koff[kKu];
+    const uint8_t* const vbase = a.vc + (page0 * a.Hkv + h) * a.bs * a.hd;
+    uint32_t koff[kKu], voff;
 #pragma unroll
     for (int u = 0; u < kKu; ++u) {
-        const int key = (lid + u * 256) / (HD / 16) & 15, d = (lid + u * 256) % (HD / 16) * 16;
+        const int key = (tid + u * 256) / (HD / 16) & 15, d = (tid + u * 256) % (HD / 16) * 16;
         koff[u] = key * a.hd + (d < a.hd ? d : 0);
     }
+    voff = (vk & 8) * a.hd + (vd < a.hd ? vd : 0);
+    const auto byte_at = [](const uint8_t* p) {  // the dword around it, by the scalar unit
+        const auto w = reinterpret_cast<uintptr_t>(p);
+        return (*reinterpret_cast<uniform_int*>(w & ~uintptr_t{3}) >> ((w & 3) * 8)) & 255;
+    };
     uint32_t kraw[kKu][4], vraw[8];
-    int kb[kKu], vb = 0, vphys = -1, vfound = -1, vin = 0, kphys[kKu], kin[kKu];
+    int kb[kKu], vb = 0, vphys = -1, vfound = -1, vin = 0, kfound[kKu], kin[kKu];
     const auto find = [&](int step) {
-        const int key0 = base32 + step * KT;
-        if (has_k) {
 #pragma unroll
-            for (int u = 0; u < kKu; ++u) kphys[u] = page_of(key0 + ((lid + u * 256) / (HD / 16) & ~15), kin[u]);
-        }
-        // every lane, as it also says which blocks of the tile have a page
-        vfound = page_of(key0 + ((kAllV || vk < KT ? vk : 0) & ~15), vin);
+        for (int u = 0; u < kKu; ++u) kfound[u] = page_of(base32 + step * KT + k_block(u) * 16, kin[u]);
+        vfound = page_of(base32 + step * KT + v_block * 16, vin);
     };
     const auto load = [&] {
         vphys = vfound;
-        if (has_k) {
 #pragma unroll
-            for (int u = 0; u < kKu; ++u) {
-                const uint32_t pg = max(kphys[u], 0);
-                load_words<4>(kraw[u], kbase + static_cast<uint64_t>(pg) * page_bytes + (kin[u] * a.hd + koff[u]));
-                kb[u] = ksc[static_cast<uint64_t>(pg) * static_cast<uint32_t>(a.Hkv)];
-            }
+        for (int u = 0; u < kKu; ++u) {
+            const int64_t pg = max(kfound[u], 0);
+            load_words<4>(kraw[u], kbase + pg * page_bytes + kin[u] * a.hd + koff[u]);
+            kb[u] = byte_at(a.ks + (page0 + pg) * a.Hkv + h);
         }
-        if (!kRoles || wave >= 4) {
-            const uint32_t pg = max(vphys, 0);
-            const uint8_t* p = vbase + static_cast<uint64_t>(pg) * page_bytes + vin * a.hd;
+        const int64_t pg = max(vphys, 0);
+        const uint8_t* const p = vbase + pg * page_bytes + vin * a.hd;
 #pragma unroll
-            for (int i = 0; i < 8; ++i, p += a.hd) load_words<1>(&vraw[i], p);
-            vb = vsc[static_cast<uint64_t>(pg) * static_cast<uint32_t>(a.Hkv)];
-        }
+        for (int i = 0; i < 8; ++i) load_words<1>(&vraw[i], p + i * a.hd + voff);
+        vb = byte_at(a.vs + (page0 + pg) * a.Hkv + h);
     };
     const auto store = [&](int step, int buf) {
-        if (has_k) {
 #pragma unroll
-            for (int u = 0; u < kKu; ++u) {
-                const int key = (lid + u * 256) / (HD / 16), c = (lid + u * 256) % (HD / 16) * 2;
-                const float scale = e8_scale(kb[u]);
+        for (int u = 0; u < kKu; ++u) {
+            const int key = (tid + u * 256) / (HD / 16), c = (tid + u * 256) % (HD / 16) * 2;
+            const float scale = e8_scale(kb[u]);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const h2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i], scale, false);
-                    const h2 x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i], scale, true);
-                    const h2 x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i + 1], scale, false);
-                    const h2 x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i + 1], scale, true);
-                    *reinterpret_cast<h8*>(&s_k[buf][key * HD + k_piece(key, c + i) * 8]) =
-                        h8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
-                }
+            for (int i = 0; i < 2; ++i) {
+                const h2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i], scale, false);
+                const h2 x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i], scale, true);
+                const h2 x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i + 1], scale, false);
+                const h2 x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i + 1], scale, true);
+                *reinterpret_cast<h8*>(&s_k[buf][key * HD + k_piece(key, c + i) * 8]) =
+                    h8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
+            }
+        }
+        // V: what no row may see is zero, whatever it holds, and NaN is zero with its place kept
+        // in s_bits
+        const int tile0 = base32 + step * KT, key0 = tile0 + vk;
+        float scale = e8_scale(vb);
+        uint32_t nan = vb == 255 ? 0x80u : 0u, bits = 0;
+        if (tile0 + KT > hi32 || tile0 < lo32 || vphys < 0) {
+            const bool ok = vphys >= 0 && key0 < hi32 && key0 + 8 > lo32;
+            if (!ok) scale = 1.0f, nan = 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (!ok || key0 + i >= hi32 || key0 + i < lo32) vraw[i] = 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) nan |= (vraw[i] & 0x7F7F7F7Fu) + 0x01010101u;
+        if (__any(nan & 0x80808080u)) {
+            const bool all_nan = __builtin_bit_cast(uint32_t, scale) >> 23 == 255;
+            if (all_nan) scale = 1.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool in = key0 + i < hi32 && key0 + i >= lo32;
+                const uint32_t n = all_nan ? (in ? ~0u : 0u) : nan_bytes(vraw[i]);
+                bits |= (n & 0x01010101u) << i;
+                vraw[i] &= ~n;
             }
         }
         if (has_v) {
-            // what no row may see is zero, whatever it holds, and NaN is zero with its place
-            // kept in s_bits
-            const int tile0 = base32 + step * KT, key0 = tile0 + vk;
-            float scale = e8_scale(vb);
-            uint32_t nan = vb == 255 ? 0x80u : 0u, bits = 0;
-            if (tile0 + KT > hi32 || tile0 < lo32 || __any(vphys < 0)) {
-                const bool ok = vphys >= 0 && key0 < hi32 && key0 + 8 > lo32;
-                if (!ok) scale = 1.0f, nan = 0;
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (!ok || key0 + i >= hi32 || key0 + i < lo32) vraw[i] = 0;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) nan |= (vraw[i] & 0x7F7F7F7Fu) + 0x01010101u;
-            if (nan & 0x80808080u) {
-                const bool all_nan = __builtin_bit_cast(uint32_t, scale) >> 23 == 255;
-                if (all_nan) scale = 1.0f;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const bool in = key0 + i < hi32 && key0 + i >= lo32;
-                    const uint32_t n = all_nan ? (in ? ~0u : 0u) : nan_bytes(vraw[i]);
-                    bits |= (n & 0x01010101u) << i;
-                    vraw[i] &= ~n;
-                }
-            }
             uint32_t w[4][4];  // [d][pair of keys]
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -303,10 +301,13 @@ __global__ __launch_bounds__(WAVES * 64, HD > 128 ? WAVES / 4 : 2) void kv8_prom
 #pragma unroll
             for (int ks = 0; ks < kSub; ++ks)
 #pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(sc[ks][i], a.c, ref));
-                    l += w;
-                    p[ks * 2 + (i >> 3)][i & 7] = (half_t)w;
+                for (int i = 0; i < 16; i += 2) {
+                    const h2 w = {(half_t)__builtin_amdgcn_exp2f(fmaf(sc[ks][i], a.c, ref)),
+                                  (half_t)__builtin_amdgcn_exp2f(fmaf(sc[ks][i + 1], a.c, ref))};
+                    p[ks * 2 + (i >> 3)][i & 7] = w[0];
+                    p[ks * 2 + (i >> 3)][(i & 7) + 1] = w[1];
+                    // their sum, of the weights as rounded
+                    l = __builtin_amdgcn_fdot2(w, h2{(half_t)1.0f, (half_t)1.0f}, l, false);
                 }
 #pragma unroll
             for (int j = 0; j < kDt; ++j) {
@@ -348,42 +349,71 @@ __global__ __launch_bounds__(WAVES * 64, HD > 128 ? WAVES / 4 : 2) void kv8_prom
     }
 
     l += __shfl_xor(l, 32, kWave);
-    const auto out_row = [&](int r) {  // of the tile, and whether it is live
+    const auto out_row = [&](int r) {  // of row r of the tile
         const int rr = t.r0 + r, rs = rr / a.G;
-        const int64_t rp = t.sp + rs;
-        half_t* const to = a.out + (tok0 + rs) * a.os + (h * a.G + rr - rs * a.G) * a.hd;
-        return std::pair<half_t*, bool>(to, rp >= 0 && rp < t.sl);
+        return a.out + (tok0 + rs) * a.os + (h * a.G + rr - rs * a.G) * a.hd;
     };
     if (t.used <= 1) {
-        if (!mine) return;
-        const auto [to, on] = out_row(wave * 32 + col);
-        const bool some = on && l != 0.0f;
+        // By way of LDS, half of d at a time, so that a row leaves in runs of 16 bytes and more.
+        const bool some = live && l != 0.0f;
         const float inv = some ? 1.0f / l : 0.0f;
+        constexpr int kPitch = HD / 2 + 8;  // halves of a row, off the banks of the one before
+        static_assert(kPromptRows * kPitch * 2 <= 4 * kTileBytes, "the rows fit");
+        half_t* const rows = reinterpret_cast<half_t*>(s_mem) + wave * 32 * kPitch;
+        typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+        const bool vec = (reinterpret_cast<uintptr_t>(a.out) & 15) == 0 && (a.os & 7) == 0;
 #pragma unroll
-        for (int j = 0; j < kDt; ++j)
+        for (int part = 0; part < 2; ++part) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int d = j * 32 + (i >> 2) * 8 + hf * 4 + (i & 3);
-                if (d < a.hd) to[d] = (half_t)(some ? o[j][i] * inv : 0.0f);
+            for (int jj = 0; jj < kDt / 2; ++jj)
+#pragma unroll
+                for (int i = 0; i < 16; i += 4) {
+                    const int j = part * (kDt / 2) + jj;
+                    h4 v;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = (half_t)(some ? o[j][i + e] * inv : 0.0f);
+                    *reinterpret_cast<h4*>(rows + col * kPitch + jj * 32 + (i >> 2) * 8 + hf * 4) = v;
+                }
+            __builtin_amdgcn_wave_barrier();  // a wave's own rows: its LDS accesses keep their order
+#pragma unroll
+            for (int i = 0; i < 32 * HD / 2 / 8 / 64; ++i) {
+                const int u = i * 64 + lane, r = u / (HD / 16), d = u % (HD / 16) * 8, dd = part * (HD / 2) + d;
+                const h8 v = *reinterpret_cast<const h8*>(rows + r * kPitch + d);
+                if (wave * 32 + r < t.rows && dd < a.hd) {
+                    half_t* const to = out_row(wave * 32 + r) + dd;
+                    if (vec) {
+                        *reinterpret_cast<h8*>(to) = v;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) to[e] = v[e];
+                    }
+                }
             }
+            __builtin_amdgcn_wave_barrier();
+        }
         return;
     }
-    // partial sums [split][d, maximum, sum][row]
+    // Partial sums [split][row][hd], then the rows' maxima and sums of weights; written through to
+    // memory and read from there (agent scope), joined by the tile's last workgroup in their order.
     const int64_t group = (b * a.tiles[g] + tile) * a.Hkv + h;
-    const int64_t apart = static_cast<int64_t>(kRowsT) * (a.hd + 2);
+    const int64_t apart = static_cast<int64_t>(kPromptRows) * (a.hd + 2);
     float* const part = a.part + a.part0[g] + group * a.nsplit[g] * apart;
     {
-        float* const to = part + split * apart + wave * 32 + col;
+        const int r = wave * 32 + col;
+        float* const to = part + split * apart + static_cast<int64_t>(r) * a.hd;
+        float* const ml = part + split * apart + static_cast<int64_t>(kPromptRows) * a.hd + 2 * r;
 #pragma unroll
         for (int j = 0; j < kDt; ++j)
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const int d = j * 32 + (i >> 2) * 8 + hf * 4 + (i & 3);
-                if (d < a.hd) store_agent(to + d * kRowsT, o[j][i]);
+            for (int i = 0; i < 16; i += 4) {
+                const int d = j * 32 + (i >> 2) * 8 + hf * 4;
+                if (d < a.hd)
+                    st8_stream_wt(reinterpret_cast<half_t*>(to + d),
+                                  __builtin_bit_cast(h8, f4{o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]}));
             }
         if (hf == 0) {
-            store_agent(to + a.hd * kRowsT, m);
-            store_agent(to + (a.hd + 1) * kRowsT, l);
+            store_agent(ml, m);
+            store_agent(ml + 1, l);
         }
     }
     __builtin_amdgcn_s_waitcnt(kDrainVmem);
@@ -394,47 +424,54 @@ __global__ __launch_bounds__(WAVES * 64, HD > 128 ? WAVES / 4 : 2) void kv8_prom
                  static_cast<unsigned>(t.used - 1);
     __syncthreads();
     if (!s_last) return;
-    if (tid == 0) *counter = 0;
-    const int r = tid & (kRowsT - 1);
-    if (r >= t.rows) return;
-    const float* const from = part + r;
-    float mm = -INFINITY, tot = 0.0f;
-    for (int sp = 0; sp < t.used; ++sp) mm = fmaxf(mm, load_agent(from + sp * apart + a.hd * kRowsT));
-    const float ref = mm == -INFINITY ? 0.0f : mm;
-    const auto weight = [&](int sp) {
-        return join_weight(load_agent(from + sp * apart + a.hd * kRowsT),
-                           load_agent(from + sp * apart + (a.hd + 1) * kRowsT), ref);
-    };
-    for (int sp = 0; sp < t.used; ++sp)
-        tot = fmaf(load_agent(from + sp * apart + (a.hd + 1) * kRowsT), weight(sp), tot);
-    const auto [to, on] = out_row(r);
-    const bool some = on && tot != 0.0f;
-    for (int d = tid / kRowsT * 8; d < a.hd; d += 16) {  // two lanes per row
+    if (tid == 0) *counter = 0;  // for the next call
+    float* const w_of = reinterpret_cast<float*>(s_mem);  // [split][row]: what a split's sums count
+    static_assert((kPromptSplits + 1) * kPromptRows * 4 <= 4 * kTileBytes, "the weights of kPromptSplits splits fit");
+    float* const tot_of = w_of + kPromptSplits * kPromptRows;
+    if (tid < kPromptRows) {
+        const float* const ml = part + static_cast<int64_t>(kPromptRows) * a.hd + 2 * tid;
+        float mm = -INFINITY, tot = 0.0f;
+        for (int sp = 0; sp < t.used; ++sp) mm = fmaxf(mm, load_agent(ml + sp * apart));
+        const float ref = mm == -INFINITY ? 0.0f : mm;
+        for (int sp = 0; sp < t.used; ++sp) {
+            const float l1 = load_agent(ml + sp * apart + 1), by = join_weight(load_agent(ml + sp * apart), l1, ref);
+            w_of[sp * kPromptRows + tid] = by;
+            tot = fmaf(l1, by, tot);
+        }
+        const int64_t rp = t.sp + (t.r0 + tid) / a.G;
+        tot_of[tid] = rp >= 0 && rp < t.sl ? tot : 0.0f;
+    }
+    __syncthreads();
+    const int pieces = a.hd >> 3;  // of eight d
+    const float inv_pieces = 1.0f / static_cast<float>(pieces);
+    for (int i = tid; i < t.rows * pieces; i += 256) {
+        const int r = small_div(i, inv_pieces), d = (i - r * pieces) * 8;
+        const uint64_t* const from = reinterpret_cast<const uint64_t*>(part + static_cast<int64_t>(r) * a.hd + d);
         float sum[8] = {};
         for (int sp = 0; sp < t.used; ++sp) {
-            const float w = weight(sp);
-            float v[8];
+            const float w = w_of[sp * kPromptRows + r];
+            uint64_t v[4];
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] = load_agent(from + sp * apart + (d + e) * kRowsT);
+            for (int e = 0; e < 4; ++e)
+                v[e] = __hip_atomic_load(from + sp * (apart / 2) + e, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) sum[e] = fmaf(v[e], w, sum[e]);
+            for (int e = 0; e < 4; ++e) {
+                sum[2 * e] = fmaf(__builtin_bit_cast(float, static_cast<uint32_t>(v[e])), w, sum[2 * e]);
+                sum[2 * e + 1] = fmaf(__builtin_bit_cast(float, static_cast<uint32_t>(v[e] >> 32)), w, sum[2 * e + 1]);
+            }
         }
+        const float tot = tot_of[r];
+        half_t* const to = out_row(r) + d;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) to[d + e] = (half_t)(some ? sum[e] / tot : 0.0f);
+        for (int e = 0; e < 8; ++e) to[e] = (half_t)(tot != 0.0f ? sum[e] / tot : 0.0f);
     }
 }
 
-template <int WAVES>
-static void prompt_go(const Kv8Attn& a, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(a.first[a.sg.n])), block(WAVES * 64);
-    if (a.hd <= 64) kv8_prompt_kernel<64, WAVES><<<grid, block, 0, s>>>(a);
-    else if (a.hd <= 128) kv8_prompt_kernel<128, WAVES><<<grid, block, 0, s>>>(a);
-    else kv8_prompt_kernel<256, WAVES><<<grid, block, 0, s>>>(a);
-}
-
 void kv8_prompt_launch(const Kv8Attn& a, hipStream_t s) {
-    if (a.rows == 256) prompt_go<8>(a, s);
-    else prompt_go<4>(a, s);
+    const dim3 grid(static_cast<unsigned>(a.first[a.sg.n])), block(256);
+    if (a.hd <= 64) kv8_prompt_kernel<64><<<grid, block, 0, s>>>(a);
+    else if (a.hd <= 128) kv8_prompt_kernel<128><<<grid, block, 0, s>>>(a);
+    else kv8_prompt_kernel<256><<<grid, block, 0, s>>>(a);
 }
 
 }  // namespace mi
