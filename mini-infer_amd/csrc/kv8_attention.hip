@@ -229,7 +229,7 @@ __global__ __launch_bounds__(Tile<HD>::kWaves * 64, 2) void kv8_attn_kernel(Kv8A
 #pragma unroll
         for (int i = 1; i < KL; ++i) mx = fmaxf(mx, x[i]);
         const float mn = fmaxf(m, max_over_groups(mx));
-        if (__any(mn > m)) {
+        if (__any(mn > m + kSlack)) {
             const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
             l *= by;
 #pragma unroll

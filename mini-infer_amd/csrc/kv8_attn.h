@@ -8,8 +8,8 @@ namespace mi {
 
 typedef float f4 __attribute__((ext_vector_type(4)));
 
-constexpr float kPShift = 14.0f;  // the softmax's weights are rounded to fp16 times 2^14
-constexpr float kSlack = 1.5f;   // how far a maximum may rise before the sums are scaled again
+constexpr float kPShift = 10.0f;  // the softmax's weights are rounded to fp16 times 2^10
+constexpr float kSlack = 5.0f;   // how far, in powers of two, a maximum may rise before the sums are scaled again
 constexpr int kMaxSplits = 64;
 
 struct Kv8Attn {

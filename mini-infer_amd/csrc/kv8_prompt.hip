@@ -44,13 +44,13 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     constexpr int kSteps = HD / 16;           // MFMA steps of q . k
     constexpr int kDt = HD / 32;              // 32-wide tiles of d
     constexpr int kKu = KT * HD / 16 / 256;   // 16-byte units of K a lane converts
-    constexpr bool kAllV = KT / 8 * (HD / 4) >= 256;
     constexpr int kTileBytes = KT * HD * 2;
     // two tiles of K and of V; afterwards the rows of the output
     __shared__ __attribute__((aligned(16))) uint8_t s_mem[4 * kTileBytes];
     const auto s_k = reinterpret_cast<half_t(*)[KT * HD]>(s_mem);
     const auto s_v = reinterpret_cast<half_t(*)[KT * HD]>(s_mem + 2 * kTileBytes);
-    __shared__ int s_ok[2][KT / 16], s_nan[2];
+    __shared__ int s_ok[2][KT / 16];
+    __shared__ __attribute__((aligned(8))) int s_mark[2][2];  // the tile that has a block without a page; that has a NaN
     __shared__ __attribute__((aligned(4))) uint8_t s_bits[2][KT / 8][HD];  // V's NaN: a bit per key
     __shared__ bool s_last;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -108,53 +108,47 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
         return key < hi32 && static_cast<uint32_t>(phys) < static_cast<uint32_t>(nb) ? phys : -1;
     };
 
-    // What a wave brings of a tile: units of 16 bytes of a key of K, four d of eight keys of V.  Its
-    // keys of a unit lie in one 16-key block, so that the block's page, scale and place are found by
-    // the scalar unit, and a lane adds an offset that never changes.
-    const int vk = kAllV ? tid / (HD / 4) * 8 : wave * 16 + (lane >> 4 & 1) * 8, vd = tid % (HD / 4) * 4;
-    const bool has_v = kAllV || lane < 32;  // (heads of 64: half of a wave brings a block of V)
-    const auto k_block = [&](int u) { return (wave * 64 + u * 256) / (HD / 16) >> 4; };
-    const int v_block = kAllV ? wave * 64 / (HD / 4) * 8 >> 4 : wave;
+    // What a wave brings of a tile: of one 16-key block (half of one where a tile has two) K in units
+    // of 16 bytes of a key, and V in units of four d of eight keys.  The block's page, scales and place
+    // are found by the scalar unit, once for both; a lane adds offsets that never change.
+    constexpr int kBlocks = KT / 16, kOwn = 4 / kBlocks;  // blocks of a tile; waves of a block
+    constexpr int kKeysW = 16 / kOwn;                      // keys of a wave
+    static_assert(kBlocks * kOwn == 4 && kKeysW * HD / 16 == 64 * kKu, "four waves bring a tile");
+    const int blk = wave / kOwn, kw = wave % kOwn * kKeysW;  // the wave's block, its first key there
+    const int vk = kKeysW == 16 ? (lane / (HD / 4) & 1) * 8 : 0, vd = lane % (HD / 4) * 4;  // of the wave's keys
+    const bool has_v = HD >= 128 || lane < 32;  // heads of 64: 32 lanes hold 16 keys of V
     const int64_t page_bytes = static_cast<int64_t>(a.Hkv) * a.bs * a.hd;
-    const uint8_t* const kbase = a.kc + (page0 * a.Hkv + h) * a.bs * a.hd;
-    const uint8_t* const vbase = a.vc + (page0 * a.Hkv + h) * a.bs * a.hd;
-    uint32_t koff[kKu], voff;
+    const uint8_t* const kbase = a.kc + (page0 * a.Hkv + h) * a.bs * a.hd + kw * a.hd;
+    const uint8_t* const vbase = a.vc + (page0 * a.Hkv + h) * a.bs * a.hd + kw * a.hd;
+    uint32_t koff[kKu];
 #pragma unroll
     for (int u = 0; u < kKu; ++u) {
-        const int key = (tid + u * 256) / (HD / 16) & 15, d = (tid + u * 256) % (HD / 16) * 16;
+        const int key = (lane + u * 64) / (HD / 16), d = (lane + u * 64) % (HD / 16) * 16;
         koff[u] = key * a.hd + (d < a.hd ? d : 0);
     }
-    voff = (vk & 8) * a.hd + (vd < a.hd ? vd : 0);
+    const uint32_t voff = vk * a.hd + (vd < a.hd ? vd : 0);
     const auto byte_at = [](const uint8_t* p) {  // the dword around it, by the scalar unit
         const auto w = reinterpret_cast<uintptr_t>(p);
         return (*reinterpret_cast<uniform_int*>(w & ~uintptr_t{3}) >> ((w & 3) * 8)) & 255;
     };
     uint32_t kraw[kKu][4], vraw[8];
-    int kb[kKu], vb = 0, vphys = -1, vfound = -1, vin = 0, kfound[kKu], kin[kKu];
-    const auto find = [&](int step) {
-#pragma unroll
-        for (int u = 0; u < kKu; ++u) kfound[u] = page_of(base32 + step * KT + k_block(u) * 16, kin[u]);
-        vfound = page_of(base32 + step * KT + v_block * 16, vin);
-    };
+    int kb = 0, vb = 0, phys = -1, found = -1, in_page = 0;
+    const auto find = [&](int step) { found = page_of(base32 + step * KT + blk * 16, in_page); };
     const auto load = [&] {
-        vphys = vfound;
+        phys = found;
+        const int64_t pg = max(found, 0), at = pg * page_bytes + in_page * a.hd;
 #pragma unroll
-        for (int u = 0; u < kKu; ++u) {
-            const int64_t pg = max(kfound[u], 0);
-            load_words<4>(kraw[u], kbase + pg * page_bytes + kin[u] * a.hd + koff[u]);
-            kb[u] = byte_at(a.ks + (page0 + pg) * a.Hkv + h);
-        }
-        const int64_t pg = max(vphys, 0);
-        const uint8_t* const p = vbase + pg * page_bytes + vin * a.hd;
+        for (int u = 0; u < kKu; ++u) load_words<4>(kraw[u], kbase + at + koff[u]);
+        kb = byte_at(a.ks + (page0 + pg) * a.Hkv + h);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) load_words<1>(&vraw[i], p + i * a.hd + voff);
+        for (int i = 0; i < 8; ++i) load_words<1>(&vraw[i], vbase + at + i * a.hd + voff);
         vb = byte_at(a.vs + (page0 + pg) * a.Hkv + h);
     };
     const auto store = [&](int step, int buf) {
 #pragma unroll
         for (int u = 0; u < kKu; ++u) {
-            const int key = (tid + u * 256) / (HD / 16), c = (tid + u * 256) % (HD / 16) * 2;
-            const float scale = e8_scale(kb[u]);
+            const int key = blk * 16 + kw + (lane + u * 64) / (HD / 16), c = (lane + u * 64) % (HD / 16) * 2;
+            const float scale = e8_scale(kb);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
                 const h2 x0 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i], scale, false);
@@ -167,11 +161,11 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
         }
         // V: what no row may see is zero, whatever it holds, and NaN is zero with its place kept
         // in s_bits
-        const int tile0 = base32 + step * KT, key0 = tile0 + vk;
+        const int tile0 = base32 + step * KT, vkey = blk * 16 + kw + vk, key0 = tile0 + vkey;
         float scale = e8_scale(vb);
         uint32_t nan = vb == 255 ? 0x80u : 0u, bits = 0;
-        if (tile0 + KT > hi32 || tile0 < lo32 || vphys < 0) {
-            const bool ok = vphys >= 0 && key0 < hi32 && key0 + 8 > lo32;
+        if (tile0 + KT > hi32 || tile0 < lo32 || phys < 0) {
+            const bool ok = phys >= 0 && key0 < hi32 && key0 + 8 > lo32;
             if (!ok) scale = 1.0f, nan = 0;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -207,11 +201,12 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<u4*>(&s_v[buf][(vd + i) * KT + v_piece<KT>(vd + i, vk >> 3) * 8]) =
+                *reinterpret_cast<u4*>(&s_v[buf][(vd + i) * KT + v_piece<KT>(vd + i, vkey >> 3) * 8]) =
                     u4{w[i][0], w[i][1], w[i][2], w[i][3]};
-            if (vd == 0 && (vk & 8) == 0) s_ok[buf][vk >> 4] = vphys >= 0;
-            *reinterpret_cast<uint32_t*>(&s_bits[buf][vk >> 3][vd]) = bits;
-            if (bits) s_nan[buf] = step;
+            *reinterpret_cast<uint32_t*>(&s_bits[buf][vkey >> 3][vd]) = bits;
+            if (vd == 0) s_ok[buf][blk] = phys >= 0;
+            if (phys < 0) s_mark[buf][0] = step;
+            if (bits) s_mark[buf][1] = step;
         }
     };
 
@@ -220,7 +215,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     for (int j = 0; j < kDt; ++j) o[j] = f16v(0);
     float m = -INFINITY, l = 0.0f;
     int step = split * t.per;
-    if (tid < 2) s_nan[tid] = -1;
+    if (tid < 4) s_mark[tid >> 1][tid & 1] = -1;
     __syncthreads();
     if (step < end) {
         find(step);
@@ -266,10 +261,9 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
                 order<kMfma>(1);
                 order<kDsRead>(1);
             }
-            int in_cache = 1;
-#pragma unroll
-            for (int i = 0; i < KT / 16; ++i) in_cache &= s_ok[buf][i];
-            const bool masked = key0 + KT > all_hi || key0 < all_lo || __builtin_amdgcn_readfirstlane(in_cache) == 0;
+            const bool masked = key0 + KT > all_hi || key0 < all_lo ||
+                                __builtin_amdgcn_readfirstlane(s_mark[buf][0]) == step;
+            const bool marked = __builtin_amdgcn_readfirstlane(s_mark[buf][1]) == step;
             if (masked) {
 #pragma unroll
                 for (int ks = 0; ks < kSub; ++ks)
@@ -288,7 +282,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
             pair_xor32(__builtin_bit_cast(uint32_t, mx), pa, pb);
             mx = fmaxf(__builtin_bit_cast(float, pa), __builtin_bit_cast(float, pb));
             const float mn = fmaxf(m, mx * a.c);  // a.c > 0
-            // the reference follows the maximum only where the weights would grow past 2^15.5
+            // the reference follows the maximum only where the weights would grow past 2^15
             if (__any(mn > m + kSlack)) {
                 const float by = m == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(m - mn);
                 l *= by;
@@ -321,7 +315,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
                 order<kMfma>(1);
                 order<kDsRead>(1);
             }
-            if (__builtin_amdgcn_readfirstlane(s_nan[buf]) == step) {  // rare: a NaN reaches the rows that see its key, and no other
+            if (marked) {  // rare: a NaN reaches the rows that see its key, and no other
                 uint8_t see[KT / 8];
 #pragma unroll
                 for (int c = 0; c < KT / 8; ++c) {

@@ -79,8 +79,8 @@ def attention(q, kc, vc, ks, vs, layer, segments, scale, window, out):
     """(out, tolerance) in 64 bits; `out` holds what rows outside the segments keep.
 
     The tolerance, per element with w the softmax's weights, n the keys, A = sum w |v|:
-      fp16 weights: 2^-11 A, and 2^-39 max|v| for each of those too small for 11 bits (2^-25 on a
-        scale of 2^14; the weights' sum is at least the largest one's, 1);
+      fp16 weights: 2^-11 A, and 2^-35 max|v| for each of those too small for 11 bits (2^-25 on a
+        scale of 2^10 or more for the largest weight; the weights' sum is at least that one's, 1);
       scores in fp32: each weight is off by the exponent's error, at most
         (hd + 4) 2^-24 scale sum |q k| <= d, in the weight and in the sum: 2 d A; the
         hardware's exp2 and the factor log2(e): 2^-21 each, of the exponent's size;
@@ -119,7 +119,7 @@ def attention(q, kc, vc, ks, vs, layer, segments, scale, window, out):
                     big = (np.abs(k) @ np.abs(x) * abs(scale)).max()
                     d = (hd + 4) * 2.0 ** -24 * big + 2.0 ** -21 * (1 + big)
                     tol[t, h] = (A * (2.0 ** -11 + 2 * d + 2 * n * 2.0 ** -24)
-                                 + n * 2.0 ** -39 * np.nan_to_num(np.abs(v)).max() + 2.0 ** -11 * np.abs(out[t, h]) + 2.0 ** -25)
+                                 + n * 2.0 ** -35 * np.nan_to_num(np.abs(v)).max() + 2.0 ** -11 * np.abs(out[t, h]) + 2.0 ** -25)
     return out, tol
 
 
