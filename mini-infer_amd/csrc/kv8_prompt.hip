@@ -20,13 +20,15 @@ typedef const __attribute__((address_space(4))) int uniform_int;  // read throug
 template <int HD>
 constexpr int prompt_keys() { return HD > 128 ? 32 : 64; }
 
-// 16-byte pieces of a row of K [key][HD] and of V^T [d][keys] are exchanged within groups of
-// eight (four for rows of 64 bytes) so that lanes on consecutive rows fall on different banks.
-__device__ __forceinline__ int k_piece(int key, int c) { return c ^ ((key & 3) | ((key >> 1) & 4)); }
+// LDS reads 256 bytes a clock, 16 lanes of 16 bytes.  The 16-byte pieces of a row of K [key][HD] and
+// of V^T [d][KT] are exchanged within the row so that 16 lanes on consecutive rows fall on
+// different banks (with eight lanes apart only, every read took half as long again).
+template <int HD>
+__device__ __forceinline__ int k_piece(int key, int c) { return c ^ (HD == 64 ? key >> 1 & 7 : key & 15); }
 template <int KT>
 __device__ __forceinline__ int v_piece(int d, int c) {
-    if constexpr (KT == 64) return c ^ (((d >> 2) & 7) ^ ((d & 3) << 1));
-    else return c ^ (((d >> 2) & 3) ^ (d & 2));
+    if constexpr (KT == 64) return c ^ ((d >> 1 & 7) ^ (d >> 4 & 1));
+    else return c ^ (d >> 2 & 3);
 }
 
 // The next `n` instructions of a kind, in the scheduler's order.
@@ -155,7 +157,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
                 const h2 x1 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i], scale, true);
                 const h2 x2 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i + 1], scale, false);
                 const h2 x3 = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(kraw[u][2 * i + 1], scale, true);
-                *reinterpret_cast<h8*>(&s_k[buf][key * HD + k_piece(key, c + i) * 8]) =
+                *reinterpret_cast<h8*>(&s_k[buf][key * HD + k_piece<HD>(key, c + i) * 8]) =
                     h8{x0[0], x0[1], x1[0], x1[1], x2[0], x2[1], x3[0], x3[1]};
             }
         }
@@ -238,7 +240,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
                 // row 16 i + 8 j + 4 f + e of the subtile stands for key 16 i + 8 f + 4 j + e
                 const int key = ks * 32 + (col & 0x13) + ((col & 4) << 1) + ((col & 8) >> 1);
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i) kf[ks & 1][i] = ld8(sk + key * HD + k_piece(key, 2 * i + hf) * 8);
+                for (int i = 0; i < kSteps; ++i) kf[ks & 1][i] = ld8(sk + key * HD + k_piece<HD>(key, 2 * i + hf) * 8);
             };
             const auto v_read = [&](int j) {
                 const int d = j * 32 + col;
