@@ -77,28 +77,24 @@ template <int VW>
 __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Write a) {
     constexpr int R = 4;
     const int lane = threadIdx.x & 63;
-    const int64_t task = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);
-    if (task >= a.first[a.sg.n]) return;
+    const uint32_t task = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);  // < 2^31
+    if (task >= static_cast<uint32_t>(a.first[a.sg.n])) return;
     int g = 0;
-    while (task >= a.first[g + 1]) ++g;
-    int64_t t = task - a.first[g];
+    while (task >= static_cast<uint32_t>(a.first[g + 1])) ++g;
+    uint32_t t = task - static_cast<uint32_t>(a.first[g]);
     const int which = static_cast<int>(t & 1);
     t >>= 1;
-    const int h = static_cast<int>(t % a.Hkv);
-    t /= a.Hkv;
-    const int pg = static_cast<int>(t % a.pages[g]);
-    const int64_t b = t / a.pages[g];
+    const int h = static_cast<int>(t % static_cast<uint32_t>(a.Hkv));
+    t /= static_cast<uint32_t>(a.Hkv);
+    const int pg = static_cast<int>(t % static_cast<uint32_t>(a.pages[g]));
+    const int64_t b = t / static_cast<uint32_t>(a.pages[g]);
     // the sequence's new positions [p0, p1), and this page's part of them
     const int64_t sp = a.sg.sp[g][b];
     const int64_t p0 = max<int64_t>(sp, 0), p1 = min<int64_t>(sp + a.sg.S[g], a.sg.sl[g][b]);
-    const int64_t blk = p0 / a.bs + pg;
+    const int64_t blk = static_cast<uint32_t>(p0) / static_cast<uint32_t>(a.bs) + pg;  // 0 <= p0 < 2^31
     const int64_t lo = max(p0, blk * a.bs), hi = min(p1, (blk + 1) * a.bs);
     if (lo >= hi || blk >= a.sg.mb[g]) return;
     const int64_t phys = a.sg.bt[g][b * a.sg.mb[g] + blk];
-    if (phys < 0 || phys >= a.num_blocks) return;
-    const int64_t page = (a.layer * a.num_blocks + phys) * a.Hkv + h;
-    uint8_t* const rows = a.cache[which] + page * a.bs * a.hd;
-    uint8_t* const scale = a.scale[which] + page;
     const half_t* const src = a.src[which] + (a.sg.off[g] + b * a.sg.S[g] + (lo - sp)) * a.stride[which] + h * a.hd;
     const int slot = static_cast<int>(lo - blk * a.bs), n = static_cast<int>(hi - lo);
     const int vph = a.hd / VW, nv = n * vph;
@@ -119,6 +115,11 @@ __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Write a) {
     };
 #pragma unroll
     for (int r = 0; r < R; ++r) x[r] = lane + r * 64 < nv ? load(lane + r * 64) : hv<VW>(0);
+    // the rows are asked for before the table's answer is needed
+    if (phys < 0 || phys >= a.num_blocks) return;
+    const int64_t page = (a.layer * a.num_blocks + phys) * a.Hkv + h;
+    uint8_t* const rows = a.cache[which] + page * a.bs * a.hd;
+    uint8_t* const scale = a.scale[which] + page;
     const int old = slot > 0 ? static_cast<int>(*scale) - kE8Bias : -1000;
 #pragma unroll
     for (int r = 0; r < R; ++r) take(x[r]);
@@ -235,7 +236,7 @@ extern "C" int mi_kv8_scatter_f16(const void* k, const void* v, int64_t k_stride
         a.first[i + 1] = a.first[i] + a.sg.B[i] * a.pages[i] * Hkv * 2;
     }
     const int64_t groups = ceil_div(a.first[a.sg.n], 4);
-    if (groups > kMaxGridX) return MI_ERR_UNSUPPORTED;
+    if (groups > kMaxGridX / 4) return MI_ERR_UNSUPPORTED;
     const bool vec = head_dim % 8 == 0 && aligned16(k) && aligned16(v) && aligned16(k_cache) &&
                      aligned16(v_cache) && (T == 1 || (k_stride % 8 == 0 && v_stride % 8 == 0));
     const dim3 grid(static_cast<unsigned>(groups)), block(256);
