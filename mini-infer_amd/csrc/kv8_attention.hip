@@ -23,7 +23,13 @@
 
 namespace mi {
 
-constexpr int kFewRows = 64;   // query rows of a (sequence, KV head) up to which tiles of 16 take them
+// Which of the two kernels a segment takes.  Tiles of 16 rows read every key once each, tiles of
+// 128 once for all, but need many sequences, heads or rows to fill the GPU.  Measured, tiles of 16
+// against 128 (us), by the number of 16-row tiles: head_dim 128, a prompt's chunk at 8000: 228 tiles 93 / 87,
+// 452 143 / 128; two at 2000: 232 44 / 56, 456 67 / 60; head_dim 64: 544 39 / 44, 1056 68 / 60; head_dim
+// 256, which takes tiles of 128 at a wave per SIMD: 528 63 / 78, 1040 111 / 100.
+constexpr int kFewRows = 64;  // rows of a (sequence, KV head) that always go in tiles of 16
+constexpr int64_t few_tiles(int64_t hd) { return hd <= 64 ? 700 : hd <= 128 ? 400 : 1000; }
 constexpr int kRows = 16;      // query rows of a tile: (token, head of the KV head's group)
 constexpr int64_t kWant = 1024;        // workgroups that a segment of few rows is split into
 constexpr int64_t kPromptWant = 512;   // and one of many rows
@@ -84,10 +90,12 @@ __global__ __launch_bounds__(Tile<HD>::kWaves * 64, 2) void kv8_attn_kernel(Kv8A
     int g = 0;
     while (id >= static_cast<uint32_t>(a.first[g + 1])) ++g;
     id -= static_cast<uint32_t>(a.first[g]);
+    // splits outermost: those that a short sequence leaves empty are whole runs of workgroups (every
+    // eighth of them in use, and all of those fell to a quarter of the CUs: 37 us where 18 do)
     const int h = divmod(id, a.Hkv);
-    const int split = divmod(id, a.nsplit[g]);
     const int tile = divmod(id, a.tiles[g]);
-    const int64_t b = id;
+    const int64_t b = divmod(id, static_cast<int>(a.sg.B[g]));
+    const int split = static_cast<int>(id);
     const TileKeys t = tile_keys<kRows, kKeys, L::kLeast>(a, g, b, tile);
     if (split >= max(t.used, 1)) return;
     const int col = lane & 15, grp = lane >> 4;
@@ -413,7 +421,7 @@ static int kv8_attn_plan(const Kv8Attn& all, Kv8Attn& few, Kv8Attn& many, int64_
     int64_t floats = 0, counters = 0;
     for (int i = 0; i < all.sg.n; ++i) {
         const int64_t rows = all.sg.S[i] * all.G;
-        const bool wide = rows > kFewRows;
+        const bool wide = rows > kFewRows && all.sg.B[i] * ceil_div(rows, kRows) * all.Hkv >= few_tiles(all.hd);
         Kv8Attn& a = wide ? many : few;
         const int n = a.sg.n++;
         a.sg.off[n] = all.sg.off[i];

@@ -111,5 +111,6 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
 void kv8_prompt_launch(const Kv8Attn& a, hipStream_t s);
 constexpr int kPromptRows = 128;   // query rows of its tile
 constexpr int kPromptSplits = 32;  // at most
+constexpr int kPromptLeast = 16;   // tiles of keys of a split: the join of many small ones costs more
 
 }  // namespace mi

@@ -63,11 +63,10 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     while (id >= static_cast<uint32_t>(a.first[g + 1])) ++g;
     id -= static_cast<uint32_t>(a.first[g]);
     const int h = divmod(id, a.Hkv);
-    const int split = divmod(id, a.nsplit[g]);
-    // a sequence's last tiles have the most keys: first
-    const int64_t b = id % static_cast<uint32_t>(a.sg.B[g]);
-    const int tile = a.tiles[g] - 1 - static_cast<int>(id / static_cast<uint32_t>(a.sg.B[g]));
-    const TileKeys t = tile_keys<kPromptRows, KT, 4>(a, g, b, tile);
+    const int64_t b = divmod(id, static_cast<int>(a.sg.B[g]));
+    const int tile = a.tiles[g] - 1 - divmod(id, a.tiles[g]);  // a sequence's last tiles have the most keys: first
+    const int split = static_cast<int>(id);  // outermost, as in kv8_attention.hip
+    const TileKeys t = tile_keys<kPromptRows, KT, kPromptLeast>(a, g, b, tile);
     if (split >= max(t.used, 1)) return;
     const int64_t tok0 = a.sg.off[g] + b * t.S;
 
