@@ -491,6 +491,12 @@ int mi_kv8_attention_f16(const void* q, int64_t q_stride, const void* k_cache,
                          int num_segments, void* workspace, int64_t workspace_bytes,
                          void* stream);
 
+/* Test hook (no counterpart in the reference): query rows of the tiles that
+ * mi_kv8_attention_f16 works in, 16 or 128; 0 chooses by the segments' shapes.
+ * It is part of what mi_kv8_attention_workspace_bytes goes by.  Returns the
+ * previous value. */
+int mi_kv8_attention_test_tile(int rows);
+
 /* ---- the pages of a cache ---------------------------------------------------- */
 
 /* One tensor [layers, num_blocks, page_bytes] of a paged cache: K or V of

@@ -16,6 +16,7 @@
 // of that block alone.  The same freedom in d lets a lane read K and V in runs of 16 and 8
 // bytes (head_dim 128) straight from the pages.
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 
 #include "kv8_attn.h"
@@ -30,6 +31,7 @@ namespace mi {
 // 256, which takes tiles of 128 at a wave per SIMD: 528 63 / 78, 1040 111 / 100.
 constexpr int kFewRows = 64;  // rows of a (sequence, KV head) that always go in tiles of 16
 constexpr int64_t few_tiles(int64_t hd) { return hd <= 64 ? 700 : hd <= 128 ? 400 : 1000; }
+std::atomic<int> g_kv8_tile{0};  // mi_kv8_attention_test_tile
 constexpr int kRows = 16;      // query rows of a tile: (token, head of the KV head's group)
 constexpr int64_t kWant = 1024;        // workgroups that a segment of few rows is split into
 constexpr int64_t kPromptWant = 512;   // and one of many rows
@@ -419,9 +421,11 @@ static int kv8_attn_plan(const Kv8Attn& all, Kv8Attn& few, Kv8Attn& many, int64_
     few = many = all;
     few.sg.n = many.sg.n = 0;
     int64_t floats = 0, counters = 0;
+    const int asked = g_kv8_tile.load(std::memory_order_relaxed);
     for (int i = 0; i < all.sg.n; ++i) {
         const int64_t rows = all.sg.S[i] * all.G;
-        const bool wide = rows > kFewRows && all.sg.B[i] * ceil_div(rows, kRows) * all.Hkv >= few_tiles(all.hd);
+        const int64_t tiles16 = all.sg.B[i] * ceil_div(rows, kRows) * all.Hkv;
+        const bool wide = asked == 0 ? rows > kFewRows && tiles16 >= few_tiles(all.hd) : asked != kRows;
         Kv8Attn& a = wide ? many : few;
         const int n = a.sg.n++;
         a.sg.off[n] = all.sg.off[i];
@@ -484,6 +488,11 @@ extern "C" int64_t mi_kv8_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int
     if (st != MI_OK) return st;
     const int pl = kv8_attn_plan(a, few, many, bytes);
     return pl != MI_OK ? pl : bytes;
+}
+
+extern "C" int mi_kv8_attention_test_tile(int rows) {
+    if (rows != 0 && rows != mi::kRows && rows != mi::kPromptRows) return MI_ERR_INVALID_ARGUMENT;
+    return mi::g_kv8_tile.exchange(rows);
 }
 
 extern "C" int mi_kv8_attention_f16(const void* q, int64_t q_stride, const void* k_cache,

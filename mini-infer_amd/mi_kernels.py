@@ -72,6 +72,7 @@ SIGNATURES = {
     "mi_greedy_argmax_ws_f16": [_c_void_p, _i64, _i64, _c_void_p, _c_void_p, _i64, _c_void_p],
     "mi_softmax_test_poll_limit": [_int],
     "mi_greedy_argmax_test_poll_limit": [_int],
+    "mi_kv8_attention_test_tile": [_int],
     "mi_exchange_test_mode": [_int],
     "mi_abi_version": [],
     "mi_rope_partial_qk_f16": [_c_void_p] * 6 + [_i64] * 9 + [_int, _f32, _c_void_p],
@@ -1092,6 +1093,15 @@ def kv8_attention_workspace_bytes(num_heads: int, num_kv_heads: int, head_dim: i
     if n < 0:
         _check(n, "mi_kv8_attention_workspace_bytes")
     return n
+
+
+def kv8_attention_test_tile(rows: int) -> int:
+    """Test hook: query rows of the attention's tiles, 16 or 128 (0: by the segments'
+    shapes); returns the previous value."""
+    prev = int(load_library().mi_kv8_attention_test_tile(int(rows)))
+    if prev < 0:
+        raise ValueError("rows must be 0, 16 or 128")
+    return prev
 
 
 def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, layer: int, segments, scale=None,

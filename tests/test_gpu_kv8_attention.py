@@ -11,6 +11,14 @@ pytestmark = pytest.mark.gpu
 NAN = 0x7F
 
 
+@pytest.fixture(autouse=True, params=[0, 128], ids=["by shape", "tiles of 128"])
+def tile(mk, request):
+    """Every test in the tiles that its shapes choose, and in tiles of 128 query rows."""
+    prev = mk.kv8_attention_test_tile(request.param)
+    yield request.param
+    mk.kv8_attention_test_tile(prev)
+
+
 class Case:
     """A cache, its segments and queries; pages in random order, one owner each."""
 
@@ -109,6 +117,19 @@ def test_prompts_of_some_length(mk, dev, Hq, Hkv, hd):
     c.check(mk, dev, window=129)
 
 
+@pytest.mark.parametrize("Hq,Hkv,hd,S,B", [(28, 4, 128, 65, 4), (16, 16, 64, 81, 8), (8, 4, 256, 129, 16),
+                                           (28, 4, 128, 9, 30), (8, 4, 256, 100, 3)])
+def test_either_side_of_the_choice(mk, dev, Hq, Hkv, hd, S, B):
+    """About as many tiles of 16 rows as move a segment to tiles of 128, in one call with single tokens."""
+    c = Case(S, Hq, Hkv, hd, 16, [(1, [(90, 91)]), (S, [(7 * b, 7 * b + S) for b in range(B)])]).unused()
+    c.check(mk, dev)
+    n = mk.kv8_attention_workspace_bytes(Hq, Hkv, hd, R.dev_segments(c.segs, dev))
+    prev = mk.kv8_attention_test_tile(16)
+    c.check(mk, dev)
+    mk.kv8_attention_test_tile(prev)
+    assert mk.kv8_attention_workspace_bytes(Hq, Hkv, hd, R.dev_segments(c.segs, dev)) == n
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_long_sequences_in_splits(mk, dev, hd):
     c = Case(hd, 4, 2, hd, 16, [(1, [(4999, 5000), (2300, 2301), (70, 71)])]).unused()
@@ -203,7 +224,7 @@ def test_layers_strides_and_the_binding(mk, dev):
         c.run(mk, dev, layer=3)
 
 
-def test_the_same_bits_each_time_and_in_any_company(mk, dev):
+def test_the_same_bits_each_time(mk, dev):
     """A sequence's output is the same from call to call."""
     c = Case(9, 28, 4, 128, 16, [(1, [(1500, 1501), (64, 65), (300, 301)]), (40, [(100, 140)])]).unused()
     a = c.check(mk, dev)
