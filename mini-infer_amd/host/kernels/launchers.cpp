@@ -12,6 +12,7 @@
 #include <string>
 
 #include "kernels/gelu_kernel.h"
+#include "kernels/kv8_kernel.h"
 #include "kernels/model_utils_kernel.h"
 #include "kernels/rmsnorm_kernel.h"
 #include "kernels/rope_kernel.h"
@@ -324,6 +325,97 @@ void launch_top_p_sample_batched(const __half* logits, int B, int vocab, float p
     if (B <= 0) return;
     check(mi_top_p_sample_batched_f16(logits, B, vocab, p, temperature, seed, out, sv(stream)),
           "launch_top_p_sample_batched");
+}
+
+void launch_rope_partial_qk(__half* q, __half* k, const int64_t* positions_d,
+                            const float* inv_freq_h, int T, int Hq, int Hkv, int head_dim,
+                            int rotary_dim, int64_t q_stride, int64_t k_stride, bool interleaved,
+                            float mscale, hipStream_t stream) {
+    check(mi_rope_partial_qk_f16(q, k, q, k, positions_d, inv_freq_h, T, Hq, Hkv, head_dim,
+                                 rotary_dim, q_stride, k_stride, q_stride, k_stride, interleaved,
+                                 mscale, sv(stream)),
+          "launch_rope_partial_qk");
+}
+
+void launch_kv8_scatter(const __half* k, const __half* v, uint8_t* k_cache, uint8_t* v_cache,
+                        uint8_t* k_scale, uint8_t* v_scale, const int* block_table,
+                        const int* seq_len, const int* start_pos, int B, int S, int layer,
+                        int num_blocks, int Hkv, int head_dim, int block_size,
+                        int max_blocks_per_seq, hipStream_t stream) {
+    const mi_kv_segment seg{0, B, S, block_table, seq_len, start_pos, max_blocks_per_seq};
+    const int64_t T = static_cast<int64_t>(B) * S, row = static_cast<int64_t>(Hkv) * head_dim;
+    check(mi_kv8_scatter_f16(k, v, row, row, T, Hkv, head_dim, k_cache, v_cache, k_scale, v_scale,
+                             layer, num_blocks, block_size, &seg, T > 0 ? 1 : 0, sv(stream)),
+          "launch_kv8_scatter");
+}
+
+int64_t kv8_attention_workspace_bytes(int B, int S, int Hq, int Hkv, int head_dim,
+                                      int max_blocks_per_seq) {
+    static const int any = 0;  // the tables' addresses are not read
+    const mi_kv_segment seg{0, B, S, &any, &any, &any, max_blocks_per_seq};
+    const int64_t n = mi_kv8_attention_workspace_bytes(Hq, Hkv, head_dim, &seg,
+                                                       static_cast<int64_t>(B) * S > 0 ? 1 : 0);
+    if (n < 0) check(static_cast<int>(n), "kv8_attention_workspace_bytes");
+    return n;
+}
+
+void launch_kv8_attention(const __half* q, const uint8_t* k_cache, const uint8_t* v_cache,
+                          const uint8_t* k_scale, const uint8_t* v_scale, __half* out,
+                          const int* block_table, const int* seq_len, const int* start_pos, int B,
+                          int S, int Hq, int Hkv, int head_dim, float scale, int window, int layer,
+                          int num_blocks, int block_size, int max_blocks_per_seq, void* workspace,
+                          int64_t workspace_bytes, hipStream_t stream) {
+    const mi_kv_segment seg{0, B, S, block_table, seq_len, start_pos, max_blocks_per_seq};
+    const int64_t T = static_cast<int64_t>(B) * S, row = static_cast<int64_t>(Hq) * head_dim;
+    check(mi_kv8_attention_f16(q, row, k_cache, v_cache, k_scale, v_scale, out, row, T, Hq, Hkv,
+                               head_dim, scale, window, layer, num_blocks, block_size, &seg,
+                               T > 0 ? 1 : 0, workspace, workspace_bytes, sv(stream)),
+          "launch_kv8_attention");
+}
+
+void launch_kv_copy_pages(const mi_kv_pages* caches, int num_caches, int num_blocks, const int* src,
+                          const int* dst, int n, int* status, hipStream_t stream) {
+    check(mi_kv_pages_copy(caches, num_caches, num_blocks, src, dst, n, status, sv(stream)),
+          "launch_kv_copy_pages");
+}
+
+void launch_kv_free(int* block_table, int* seq_len, int* ref_count, int B, int max_blocks_per_seq,
+                    int num_blocks, const int* rows, int n, hipStream_t stream) {
+    check(mi_kv_pages_free(block_table, seq_len, ref_count, B, max_blocks_per_seq, num_blocks, rows,
+                           n, sv(stream)),
+          "launch_kv_free");
+}
+
+void launch_kv_fork(int* block_table, int* seq_len, int* ref_count, int B, int max_blocks_per_seq,
+                    int num_blocks, const int* parents, const int* children, int n, int* status,
+                    hipStream_t stream) {
+    check(mi_kv_pages_fork(block_table, seq_len, ref_count, B, max_blocks_per_seq, num_blocks,
+                           parents, children, n, status, sv(stream)),
+          "launch_kv_fork");
+}
+
+int64_t kv_pages_workspace_bytes(int num_blocks, int n) {
+    const int64_t bytes = mi_kv_pages_workspace_bytes(num_blocks, n);
+    if (bytes < 0) check(static_cast<int>(bytes), "kv_pages_workspace_bytes");
+    return bytes;
+}
+
+void launch_kv_reserve(const mi_kv_pages* caches, int num_caches, int* block_table, int* seq_len,
+                       int* ref_count, int B, int max_blocks_per_seq, int num_blocks,
+                       int block_size, const int* rows, const int* lengths, int n, int* status,
+                       void* workspace, int64_t workspace_bytes, hipStream_t stream) {
+    check(mi_kv_pages_reserve(caches, num_caches, block_table, seq_len, ref_count, B,
+                              max_blocks_per_seq, num_blocks, block_size, rows, lengths, n, status,
+                              workspace, workspace_bytes, sv(stream)),
+          "launch_kv_reserve");
+}
+
+void launch_kv_compact(const mi_kv_pages* caches, int num_caches, int* block_table, int* ref_count,
+                       int B, int max_blocks_per_seq, int num_blocks, int* moved, void* workspace,
+                       int64_t workspace_bytes, hipStream_t stream) {
+    check(mi_kv_pages_compact(caches, num_caches, block_table, ref_count, B, max_blocks_per_seq,
+                              num_blocks, moved, workspace, workspace_bytes, sv(stream)),
+          "launch_kv_compact");
 }
 
 }  // namespace kernels
