@@ -304,7 +304,7 @@ __global__ __launch_bounds__(Tile<HD>::kWaves * 64, 2) void kv8_attn_kernel(Kv8A
         find_v(step + 2 * kWaves);
     }
 
-    // the four waves' sums, joined
+    // the waves' sums, joined
     l = sum_over_groups(l);
     if (grp == 0) {
         s_ml[wave][0][col] = m;

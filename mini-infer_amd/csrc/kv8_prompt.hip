@@ -7,6 +7,8 @@
 // 32x32x16.  As there, the scores are made transposed and their registers are the second
 // product's operand: row r of a 32-key subtile stands for the key that puts a lane's eight
 // scores of an operand in key order, so V^T is read from LDS in plain order.
+#include <type_traits>
+
 #include "kv8_attn.h"
 #include "mi_host.h"
 
@@ -14,7 +16,6 @@ namespace mi {
 
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef uint32_t u4 __attribute__((ext_vector_type(4)));
-typedef const __attribute__((address_space(4))) int uniform_int;  // read through the scalar cache
 
 // Keys of a tile: what two LDS buffers of K and V and two workgroups per CU allow.
 template <int HD>
@@ -31,6 +32,13 @@ __device__ __forceinline__ int v_piece(int d, int c) {
     else return c ^ (d >> 2 & 3);
 }
 
+// A vector register's offset, for a load relative to scalar registers: what the compiler knows to be
+// uniform it reads through the scalar cache, and a scalar load is waited for together with LDS.
+__device__ __forceinline__ uint32_t in_vgpr(uint32_t v) {
+    asm("" : "+v"(v));
+    return v;
+}
+
 // The next `n` instructions of a kind, in the scheduler's order.
 constexpr int kMfma = 0x8, kDsRead = 0x100;
 template <int KIND>
@@ -39,7 +47,7 @@ __device__ __forceinline__ void order(int n) {
     for (int i = 0; i < n; ++i) __builtin_amdgcn_sched_group_barrier(KIND, 1, 0);
 }
 
-template <int HD>
+template <int HD, bool WHOLE>
 __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8Attn a) {
     constexpr int KT = prompt_keys<HD>();
     constexpr int kSub = KT / 32;             // 32-key subtiles
@@ -55,6 +63,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     __shared__ __attribute__((aligned(8))) int s_mark[2][2];  // the tile that has a block without a page; that has a NaN
     __shared__ __attribute__((aligned(4))) uint8_t s_bits[2][KT / 8][HD];  // V's NaN: a bit per key
     __shared__ bool s_last;
+    const int hd = WHOLE ? HD : a.hd;
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int col = lane & 31, hf = lane >> 5;
@@ -82,7 +91,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     for (int i = 0; i < kSteps; ++i) {
         const int d = i * 16 + hf * 8;
         qf[i] = h8(0);
-        if (live && d < a.hd) qf[i] = ld8(a.q + (tok0 + s) * a.qs + head * a.hd + d);
+        if (live && d < hd) qf[i] = ld8(a.q + (tok0 + s) * a.qs + head * hd + d);
         if (a.neg) qf[i] = -qf[i];
     }
     // keys that every live row of the wave sees, and that any does
@@ -100,15 +109,8 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     const int base32 = static_cast<int>(t.base), lo32 = static_cast<int>(t.lo);
     const int hi32 = min(static_cast<int>(t.hi), base32 + end * KT);
     const int64_t page0 = a.layer * a.num_blocks;
+    const int last_entry = static_cast<int>((t.hi - 1) >> 4) / sub;
     const uint64_t inv_sub = ((uint64_t{1} << 40) + sub - 1) / static_cast<uint32_t>(sub);
-    const auto page_of = [&](int key, int& in_page) {  // of a 16-key block, -1 where it has none
-        const uint32_t k16 = static_cast<uint32_t>(key) >> 4;  // < 2^22, sub <= 256: the quotient is exact
-        const uint32_t idx = static_cast<uint32_t>(k16 * inv_sub >> 40);
-        in_page = static_cast<int>(k16 - idx * sub) * 16;
-        const int phys = reinterpret_cast<uniform_int*>(reinterpret_cast<uintptr_t>(table))[key < hi32 ? idx : 0];
-        return key < hi32 && static_cast<uint32_t>(phys) < static_cast<uint32_t>(nb) ? phys : -1;
-    };
-
     // What a wave brings of a tile: of one 16-key block (half of one where a tile has two) K in units
     // of 16 bytes of a key, and V in units of four d of eight keys.  The block's page, scales and place
     // are found by the scalar unit, once for both; a lane adds offsets that never change.
@@ -118,32 +120,41 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     const int blk = wave / kOwn, kw = wave % kOwn * kKeysW;  // the wave's block, its first key there
     const int vk = kKeysW == 16 ? (lane / (HD / 4) & 1) * 8 : 0, vd = lane % (HD / 4) * 4;  // of the wave's keys
     const bool has_v = HD >= 128 || lane < 32;  // heads of 64: 32 lanes hold 16 keys of V
-    const int64_t page_bytes = static_cast<int64_t>(a.Hkv) * a.bs * a.hd;
-    const uint8_t* const kbase = a.kc + (page0 * a.Hkv + h) * a.bs * a.hd + kw * a.hd;
-    const uint8_t* const vbase = a.vc + (page0 * a.Hkv + h) * a.bs * a.hd + kw * a.hd;
+    const int64_t page_bytes = static_cast<int64_t>(a.Hkv) * a.bs * hd;
+    const uint8_t* const kbase = a.kc + (page0 * a.Hkv + h) * a.bs * hd + kw * hd;
+    const uint8_t* const vbase = a.vc + (page0 * a.Hkv + h) * a.bs * hd + kw * hd;
     uint32_t koff[kKu];
 #pragma unroll
     for (int u = 0; u < kKu; ++u) {
         const int key = (lane + u * 64) / (HD / 16), d = (lane + u * 64) % (HD / 16) * 16;
-        koff[u] = key * a.hd + (d < a.hd ? d : 0);
+        koff[u] = key * hd + (d < hd ? d : 0);
     }
-    const uint32_t voff = vk * a.hd + (vd < a.hd ? vd : 0);
-    const auto byte_at = [](const uint8_t* p) {  // the dword around it, by the scalar unit
-        const auto w = reinterpret_cast<uintptr_t>(p);
-        return (*reinterpret_cast<uniform_int*>(w & ~uintptr_t{3}) >> ((w & 3) * 8)) & 255;
-    };
+    const uint32_t voff = vk * hd + (vd < hd ? vd : 0);
     uint32_t kraw[kKu][4], vraw[8];
-    int kb = 0, vb = 0, phys = -1, found = -1, in_page = 0;
-    const auto find = [&](int step) { found = page_of(base32 + step * KT + blk * 16, in_page); };
+    int kb = 0, vb = 0, phys = -1, entry = 0, in_page = 0;
+    bool in_split = false;
+    // The table's entry of the wave's block of a tile, read a tile before its page is.
+    const auto find = [&](int step) {
+        const int key = base32 + step * KT + blk * 16;
+        const uint32_t k16 = static_cast<uint32_t>(key) >> 4;  // < 2^22, sub <= 256: the quotient is exact
+        const int idx = static_cast<int>(k16 * inv_sub >> 40);
+        in_page = static_cast<int>(k16 - idx * sub) * 16;
+        in_split = key < hi32;
+        entry = *reinterpret_cast<const int*>(reinterpret_cast<const uint8_t*>(table) + in_vgpr(4u * min(idx, last_entry)));
+    };
     const auto load = [&] {
-        phys = found;
-        const int64_t pg = max(found, 0), at = pg * page_bytes + in_page * a.hd;
+        const int e = __builtin_amdgcn_readfirstlane(entry);
+        phys = in_split && static_cast<uint32_t>(e) < static_cast<uint32_t>(nb) ? e : -1;
+        const int64_t pg = max(phys, 0), at = pg * page_bytes + in_page * hd, cell = (page0 + pg) * a.Hkv + h;
+        const uint8_t *const kp = kbase + at, *const vp = vbase + at;
+        const uint32_t ko = in_vgpr(koff[0]), vo = in_vgpr(voff);
 #pragma unroll
-        for (int u = 0; u < kKu; ++u) load_words<4>(kraw[u], kbase + at + koff[u]);
-        kb = byte_at(a.ks + (page0 + pg) * a.Hkv + h);
+        for (int u = 0; u < kKu; ++u)
+            load_words<4>(kraw[u], WHOLE ? kp + ko + u * (1024 / HD) * HD : kp + in_vgpr(koff[u]));
+        kb = a.ks[cell];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) load_words<1>(&vraw[i], vbase + at + i * a.hd + voff);
-        vb = byte_at(a.vs + (page0 + pg) * a.Hkv + h);
+        for (int i = 0; i < 8; ++i) load_words<1>(&vraw[i], WHOLE ? vp + vo + i * HD : vp + in_vgpr(voff + i * hd));
+        vb = a.vs[cell];
     };
     const auto store = [&](int step, int buf) {
 #pragma unroll
@@ -233,6 +244,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
         if (some_row && key0 < any_hi && key0 + KT > any_lo) {
             // Each fragment is asked for while the products before it run: LDS answers in some
             // 100 cycles, a product takes 32.
+            const int2 mark = *reinterpret_cast<const int2*>(s_mark[buf]);
             f16v sc[kSub];
             h8 kf[2][kSteps], vf[2][kSub * 2];
             const auto k_read = [&](int ks) {
@@ -263,8 +275,8 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
                 order<kDsRead>(1);
             }
             const bool masked = key0 + KT > all_hi || key0 < all_lo ||
-                                __builtin_amdgcn_readfirstlane(s_mark[buf][0]) == step;
-            const bool marked = __builtin_amdgcn_readfirstlane(s_mark[buf][1]) == step;
+                                __builtin_amdgcn_readfirstlane(mark.x) == step;
+            const bool marked = __builtin_amdgcn_readfirstlane(mark.y) == step;
             if (masked) {
 #pragma unroll
                 for (int ks = 0; ks < kSub; ++ks)
@@ -346,7 +358,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     l += __shfl_xor(l, 32, kWave);
     const auto out_row = [&](int r) {  // of row r of the tile
         const int rr = t.r0 + r, rs = rr / a.G;
-        return a.out + (tok0 + rs) * a.os + (h * a.G + rr - rs * a.G) * a.hd;
+        return a.out + (tok0 + rs) * a.os + (h * a.G + rr - rs * a.G) * hd;
     };
     if (t.used <= 1) {
         // By way of LDS, half of d at a time, so that a row leaves in runs of 16 bytes and more.
@@ -374,7 +386,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
             for (int i = 0; i < 32 * HD / 2 / 8 / 64; ++i) {
                 const int u = i * 64 + lane, r = u / (HD / 16), d = u % (HD / 16) * 8, dd = part * (HD / 2) + d;
                 const h8 v = *reinterpret_cast<const h8*>(rows + r * kPitch + d);
-                if (wave * 32 + r < t.rows && dd < a.hd) {
+                if (wave * 32 + r < t.rows && dd < hd) {
                     half_t* const to = out_row(wave * 32 + r) + dd;
                     if (vec) {
                         *reinterpret_cast<h8*>(to) = v;
@@ -391,18 +403,18 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     // Partial sums [split][row][hd], then the rows' maxima and sums of weights; written through to
     // memory and read from there (agent scope), joined by the tile's last workgroup in their order.
     const int64_t group = (b * a.tiles[g] + tile) * a.Hkv + h;
-    const int64_t apart = static_cast<int64_t>(kPromptRows) * (a.hd + 2);
+    const int64_t apart = static_cast<int64_t>(kPromptRows) * (hd + 2);
     float* const part = a.part + a.part0[g] + group * a.nsplit[g] * apart;
     {
         const int r = wave * 32 + col;
-        float* const to = part + split * apart + static_cast<int64_t>(r) * a.hd;
-        float* const ml = part + split * apart + static_cast<int64_t>(kPromptRows) * a.hd + 2 * r;
+        float* const to = part + split * apart + static_cast<int64_t>(r) * hd;
+        float* const ml = part + split * apart + static_cast<int64_t>(kPromptRows) * hd + 2 * r;
 #pragma unroll
         for (int j = 0; j < kDt; ++j)
 #pragma unroll
             for (int i = 0; i < 16; i += 4) {
                 const int d = j * 32 + (i >> 2) * 8 + hf * 4;
-                if (d < a.hd)
+                if (d < hd)
                     st8_stream_wt(reinterpret_cast<half_t*>(to + d),
                                   __builtin_bit_cast(h8, f4{o[j][i], o[j][i + 1], o[j][i + 2], o[j][i + 3]}));
             }
@@ -424,7 +436,7 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
     static_assert((kPromptSplits + 1) * kPromptRows * 4 <= 4 * kTileBytes, "the weights of kPromptSplits splits fit");
     float* const tot_of = w_of + kPromptSplits * kPromptRows;
     if (tid < kPromptRows) {
-        const float* const ml = part + static_cast<int64_t>(kPromptRows) * a.hd + 2 * tid;
+        const float* const ml = part + static_cast<int64_t>(kPromptRows) * hd + 2 * tid;
         float mm = -INFINITY, tot = 0.0f;
         for (int sp = 0; sp < t.used; ++sp) mm = fmaxf(mm, load_agent(ml + sp * apart));
         const float ref = mm == -INFINITY ? 0.0f : mm;
@@ -437,11 +449,11 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
         tot_of[tid] = rp >= 0 && rp < t.sl ? tot : 0.0f;
     }
     __syncthreads();
-    const int pieces = a.hd >> 3;  // of eight d
+    const int pieces = hd >> 3;  // of eight d
     const float inv_pieces = 1.0f / static_cast<float>(pieces);
     for (int i = tid; i < t.rows * pieces; i += 256) {
         const int r = small_div(i, inv_pieces), d = (i - r * pieces) * 8;
-        const uint64_t* const from = reinterpret_cast<const uint64_t*>(part + static_cast<int64_t>(r) * a.hd + d);
+        const uint64_t* const from = reinterpret_cast<const uint64_t*>(part + static_cast<int64_t>(r) * hd + d);
         float sum[8] = {};
         for (int sp = 0; sp < t.used; ++sp) {
             const float w = w_of[sp * kPromptRows + r];
@@ -464,9 +476,14 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
 
 void kv8_prompt_launch(const Kv8Attn& a, hipStream_t s) {
     const dim3 grid(static_cast<unsigned>(a.first[a.sg.n])), block(256);
-    if (a.hd <= 64) kv8_prompt_kernel<64><<<grid, block, 0, s>>>(a);
-    else if (a.hd <= 128) kv8_prompt_kernel<128><<<grid, block, 0, s>>>(a);
-    else kv8_prompt_kernel<256><<<grid, block, 0, s>>>(a);
+    const auto launch = [&](auto width) {
+        constexpr int HD = decltype(width)::value;
+        if (a.hd == HD) kv8_prompt_kernel<HD, true><<<grid, block, 0, s>>>(a);
+        else kv8_prompt_kernel<HD, false><<<grid, block, 0, s>>>(a);
+    };
+    if (a.hd <= 64) launch(std::integral_constant<int, 64>{});
+    else if (a.hd <= 128) launch(std::integral_constant<int, 128>{});
+    else launch(std::integral_constant<int, 256>{});
 }
 
 }  // namespace mi
