@@ -73,6 +73,11 @@ __device__ __forceinline__ void quantise(const hv<VW>& x, float inv, float most,
 // is exchanged and no order decides a result.  VW elements per lane and access (8, or 1 for
 // heads or rows that 16-byte accesses do not fit); the first R accesses of the new rows stay
 // in registers between the maximum and the rounding.
+//
+// Bound by a chain of dependent reads (the sequence's length, the table's entry, the page's
+// exponent), each of which waits for the memory: 64 single tokens 4.1 us in a graph, 6064 tokens
+// (two prompts and 64 single tokens, 18.6 MB) 7.7 us, where a copy of as much takes 5.  The new rows are
+// asked for before the chain's answers (8.3 us otherwise).
 template <int VW>
 __global__ __launch_bounds__(256) void kv8_write_kernel(Kv8Write a) {
     constexpr int R = 4;

@@ -34,7 +34,7 @@ struct TileKeys {
     int64_t sp, sl;        // the sequence's start position and length
     int64_t lo, hi;        // keys that some live row sees
     int64_t base;          // lo, down to a block of 16
-    int steps, per, used;  // steps of 64 keys from base; steps of a split, splits in use
+    int steps, per, used;  // steps of KEYS keys from base; steps of a split, splits in use
 };
 
 // ROWS rows in a tile, KEYS keys in a step, at least LEAST steps in a split (a multiple of it).
