@@ -636,8 +636,15 @@ struct PageTable {
     int64_t NB() const { return ref.numel(); }
 };
 
-// A workspace: the caller's, or a new one (the current stream's: a call on another
-// stream is left to the wrapper, which tells the allocator).
+// A status array and a workspace: the caller's, or new ones (the current stream's: a call on
+// another stream is left to the wrapper, which makes them there).
+struct Said : Out {
+    Said(PyObject* o, const at::Tensor& on, int64_t m, PyObject* stream)
+        : Out((need(o != Py_None || stream == Py_None), o), on, at::kInt, {m}) {
+        need(t->numel() == m);
+        here(*t);
+    }
+};
 struct Scratch {
     at::Tensor made;
     const at::Tensor* t;
@@ -659,9 +666,7 @@ MI_FAST(kv_copy_pages) {
         const auto &src = ints(a[1]), &dst = ints(a[2]);
         const int64_t m = src.numel();
         need(dst.numel() == m);
-        const Out status(a[3], src, at::kInt, {m});
-        need(status.t->numel() == m);
-        here(*status.t);
+        const Said status(a[3], src, m, a[4]);
         void* s = stream_of(a[4]);
         MI_CALL(mi_kv_pages_copy, c.g, c.n, c.NB, ip(src), ip(dst), m, ip(*status.t), s);
         return status.result();
@@ -687,9 +692,7 @@ MI_FAST(kv_fork) {
         const auto &from = ints(a[3]), &to = ints(a[4]);
         const int64_t m = from.numel();
         need(to.numel() == m);
-        const Out status(a[5], from, at::kInt, {m});
-        need(status.t->numel() == m);
-        here(*status.t);
+        const Said status(a[5], from, m, a[6]);
         void* s = stream_of(a[6]);
         MI_CALL(mi_kv_pages_fork, ip(p.table), ip(p.seq), ip(p.ref), p.B(), p.mb(), p.NB(), ip(from), ip(to),
                 m, ip(*status.t), s);
@@ -706,9 +709,7 @@ MI_FAST(kv_reserve) {
         const auto &rows = ints(a[4]), &lens = ints(a[5]);
         const int64_t m = rows.numel(), bs = whole(a[6]);
         need(lens.numel() == m && c.NB == p.NB());
-        const Out status(a[7], rows, at::kInt, {m});
-        need(status.t->numel() == m);
-        here(*status.t);
+        const Said status(a[7], rows, m, a[9]);
         const Scratch w(a[8], mi_kv_pages_workspace_bytes(p.NB(), m), p.table, a[9]);
         void* s = stream_of(a[9]);
         MI_CALL(mi_kv_pages_reserve, c.g, c.n, ip(p.table), ip(p.seq), ip(p.ref), p.B(), p.mb(), p.NB(), bs,
@@ -724,9 +725,7 @@ MI_FAST(kv_compact) {
         const auto &table = ints(a[1]), &ref = ints(a[2]);
         const int64_t NB = ref.numel();
         need(table.dim() == 2 && c.NB == NB);
-        const Out moved(a[3], ref, at::kInt, {NB});
-        need(moved.t->numel() == NB);
-        here(*moved.t);
+        const Said moved(a[3], ref, NB, a[5]);
         const Scratch w(a[4], mi_kv_pages_workspace_bytes(NB, 0), table, a[5]);
         void* s = stream_of(a[5]);
         MI_CALL(mi_kv_pages_compact, c.g, c.n, ip(table), ip(ref), table.size(0), table.size(1), NB,

@@ -958,6 +958,18 @@ def _current(t, name: str) -> None:
                          f"(cuda:{_torch().cuda.current_device()})")
 
 
+def _made_on(stream):
+    """Where a wrapper makes a call's tensors: on the call's stream, so that their memory and
+    its zeros are that stream's own."""
+    torch = _torch()
+    if stream is None:
+        import contextlib  # noqa: PLC0415
+        return contextlib.nullcontext()
+    if not isinstance(stream, torch.cuda.Stream):
+        stream = torch.cuda.ExternalStream(stream.cuda_stream)
+    return torch.cuda.stream(stream)
+
+
 def _need_rows(t, name: str):
     """A [T, H, hd] fp16 GPU tensor whose tokens are contiguous rows, any distance
     apart (a slice of a fused product's rows); returns that distance."""
@@ -1127,15 +1139,15 @@ def kv8_attention(q, k_cache, v_cache, k_scale, v_scale, layer: int, segments, s
         scale = hd ** -0.5
     segs = _kv8_segments(segments)
     if out is None:
-        out = torch.zeros((T, Hq, hd), dtype=torch.float16, device=q.device)
+        with _made_on(stream):
+            out = torch.zeros((T, Hq, hd), dtype=torch.float16, device=q.device)
     os_ = _need_rows(out, "out")
     if out.shape != q.shape or out.device != q.device:
         raise ValueError("out must have q's shape and device")
     if workspace is None:
         n = kv8_attention_workspace_bytes(Hq, Hkv, hd, segments)
-        workspace = torch.zeros(max(n, 16), dtype=torch.uint8, device=q.device)
-        if stream is not None:
-            workspace.record_stream(stream)
+        with _made_on(stream):
+            workspace = torch.zeros(max(n, 16), dtype=torch.uint8, device=q.device)
     elif workspace.device != q.device or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous tensor on q's device")
     _check(load_library().mi_kv8_attention_f16(
@@ -1196,10 +1208,11 @@ def _page_state(block_table, seq_len, ref_count):
     return B, mb, ref_count.numel()
 
 
-def _status(status, n, on):
+def _status(status, n, on, stream):
     torch = _torch()
     if status is None:
-        return torch.empty(n, dtype=torch.int32, device=on.device)
+        with _made_on(stream):
+            return torch.empty(n, dtype=torch.int32, device=on.device)
     _page_ints(on, (status, "status"))
     if status.numel() != n:
         raise ValueError(f"status must hold {n} entries")
@@ -1210,9 +1223,8 @@ def _page_workspace(workspace, num_blocks, n, on, stream):
     torch = _torch()
     need = int(load_library().mi_kv_pages_workspace_bytes(num_blocks, n))
     if workspace is None:
-        workspace = torch.empty(need // 4, dtype=torch.int32, device=on.device)
-        if stream is not None:
-            workspace.record_stream(stream)
+        with _made_on(stream):
+            workspace = torch.empty(need // 4, dtype=torch.int32, device=on.device)
     elif workspace.device != on.device or not workspace.is_contiguous():
         raise ValueError("workspace must be a contiguous tensor on the cache's device")
     return workspace, workspace.numel() * workspace.element_size()
@@ -1238,7 +1250,7 @@ def kv_copy_pages(caches, src, dst, status=None, stream=None):
     if dst.numel() != n:
         raise ValueError("src and dst must have as many entries")
     arr = _page_caches(caches, None, src)
-    status = _status(status, n, src)
+    status = _status(status, n, src, stream)
     _check(load_library().mi_kv_pages_copy(arr, len(caches), caches[0].shape[1], _ptr(src),
                                            _ptr(dst), n, _ptr(status), _stream(stream)),
            "mi_kv_pages_copy")
@@ -1268,7 +1280,7 @@ def kv_fork(block_table, seq_len, ref_count, parents, children, status=None, str
     n = parents.numel()
     if children.numel() != n:
         raise ValueError("parents and children must have as many entries")
-    status = _status(status, n, block_table)
+    status = _status(status, n, block_table, stream)
     _check(load_library().mi_kv_pages_fork(_ptr(block_table), _ptr(seq_len), _ptr(ref_count), B, mb,
                                            NB, _ptr(parents), _ptr(children), n, _ptr(status),
                                            _stream(stream)), "mi_kv_pages_fork")
@@ -1290,7 +1302,7 @@ def kv_reserve(caches, block_table, seq_len, ref_count, rows, lengths, block_siz
     if lengths.numel() != n:
         raise ValueError("rows and lengths must have as many entries")
     arr = _page_caches(caches, NB, block_table)
-    status = _status(status, n, block_table)
+    status = _status(status, n, block_table, stream)
     ws, nbytes = _page_workspace(workspace, NB, n, block_table, stream)
     _check(load_library().mi_kv_pages_reserve(arr, len(caches), _ptr(block_table), _ptr(seq_len),
                                               _ptr(ref_count), B, mb, NB, block_size, _ptr(rows),
@@ -1307,7 +1319,7 @@ def kv_compact(caches, block_table, ref_count, moved=None, workspace=None, strea
         return r
     B, mb, NB = _page_state(block_table, None, ref_count)
     arr = _page_caches(caches, NB, block_table)
-    moved = _status(moved, NB, block_table)
+    moved = _status(moved, NB, block_table, stream)
     ws, nbytes = _page_workspace(workspace, NB, 0, block_table, stream)
     _check(load_library().mi_kv_pages_compact(arr, len(caches), _ptr(block_table), _ptr(ref_count),
                                               B, mb, NB, _ptr(moved), _ptr(ws), nbytes,

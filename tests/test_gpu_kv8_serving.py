@@ -144,3 +144,41 @@ def test_serving(mk, dev):
     n = int((e.h_ref > 0).sum())
     e.free([0, 1, 2, 3, 4, 5, 6, 7])
     assert n > 0 and (e.h_ref == 0).all()
+
+
+def test_what_a_call_on_another_stream_makes_is_made_there(mk, dev):
+    """With the current stream busy, calls on another one without output, workspace or status."""
+    rng = np.random.default_rng(3)
+    NBK = 64
+    cache = [R.random_cache(rng, 1, NBK, 2, 16, 64) for _ in range(2)]
+    host = [x for pair in zip(*cache) for x in pair]  # k, v, ks, vs
+    table = rng.permutation(NBK)[:2 * 31].reshape(2, 31).astype(np.int32)
+    seg = dict(token_offset=0, S=1, block_table=table, seq_len=np.array([490, 201], np.int32),
+               start_pos=np.array([489, 200], np.int32))
+    q = rng.standard_normal((3, 4, 64)).astype(np.float16)
+    d = [R.dev_cache(c, dev) for c in host[:2]] + [torch.from_numpy(c).to(dev) for c in host[2:]]
+    qd, segs = torch.from_numpy(q).to(dev), R.dev_segments([seg], dev)
+    i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=dev)
+    pages, src, dst, rows, want = torch.zeros((1, NBK, 64), device=dev), i32([1]), i32([2]), i32([0, 1]), i32([40, 20])
+    parent, child = i32([0]), i32([2])
+    state = [i32([[-1] * 4] * 3), i32([0] * 3), i32([0] * NBK)]
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        poison = torch.full((1 << 20,), 255, dtype=torch.uint8, device=dev)  # memory that the calls may be given
+        torch.cuda._sleep(20_000_000)
+        poison.fill_(255)
+        del poison
+        out = mk.kv8_attention(qd, *d, layer=0, segments=segs, stream=side)
+        said = [mk.kv_copy_pages([pages], src, dst, stream=side),
+                mk.kv_reserve([pages], *state, rows, want, 16, stream=side),
+                mk.kv_fork(*state, parent, child, stream=side)]
+        moved = mk.kv_compact([pages], state[0], state[2], stream=side)
+        with torch.cuda.stream(side):
+            got, said, moved = out.cpu().numpy(), [s.cpu().tolist() for s in said], moved.cpu().numpy()
+            mk.kv_free(*state, rows, stream=side)
+            mk.kv_free(*state, i32([2]), stream=side)
+        want_o, tol = R.attention(q, *host, 0, [seg], 64 ** -0.5, 0, np.zeros_like(q))
+        assert (np.abs(got.astype(np.float64) - want_o) <= tol).all()
+        assert said == [[0], [0, 0], [0]] and (moved[:5] >= 0).all() and (moved[5:] == -1).all()
+        torch.cuda.synchronize()
