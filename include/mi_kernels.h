@@ -473,14 +473,14 @@ int mi_kv8_scatter_f16(const void* k, const void* v, int64_t k_stride, int64_t v
  * out.  What no token sees may hold anything, NaN included.  Sums are fp32,
  * the softmax's weights are rounded to fp16.  The cached values have to be
  * within fp16's range, as mi_kv8_scatter_f16 leaves them.
- * hd a multiple of 16 (<= 256), block_size a multiple of 16 (<= 4096), at most
- * 2^25 keys per sequence, q and the caches 16-byte aligned and q_stride a
- * multiple of 8; otherwise MI_ERR_UNSUPPORTED.  out must not overlap
- * anything.  The workspace (mi_kv8_attention_workspace_bytes(Hq, Hkv, hd,
- * segments) bytes, 16-byte aligned, may be NULL when that is 0; by the
- * segments' B, S and max_blocks_per_seq alone) must hold zeros before its
- * first use and then serve only this function; calls sharing it must not
- * overlap in time. */
+ * hd a multiple of 16 (<= 256), block_size a multiple of 16 (<= 4096),
+ * Hq <= 1024, T <= 2^24, S * (Hq / Hkv) < 2^31 - 128, at most 2^25 keys per
+ * sequence, q and the caches 16-byte aligned and q_stride a multiple of 8;
+ * otherwise MI_ERR_UNSUPPORTED.  out must not overlap anything.  The workspace
+ * (mi_kv8_attention_workspace_bytes(Hq, Hkv, hd, segments) bytes, 16-byte
+ * aligned, may be NULL when that is 0; by the segments' B, S and
+ * max_blocks_per_seq alone) must hold zeros before its first use and then
+ * serve only this function; calls sharing it must not overlap in time. */
 int64_t mi_kv8_attention_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t head_dim,
                                          const mi_kv_segment* segments, int num_segments);
 int mi_kv8_attention_f16(const void* q, int64_t q_stride, const void* k_cache,

@@ -471,6 +471,8 @@ static int kv8_attn_shape(int64_t T, int64_t Hq, int64_t Hkv, int64_t hd,
     }
     if (Hkv == 0 || Hq % Hkv != 0) return MI_ERR_INVALID_ARGUMENT;
     if (hd % 16 != 0 || hd > 256 || Hq > 1024 || T > (int64_t{1} << 24)) return MI_ERR_UNSUPPORTED;
+    for (int i = 0; i < a.sg.n; ++i)  // a sequence's rows are numbered in 31 bits
+        if (a.sg.S[i] * (Hq / Hkv) > INT32_MAX - kPromptRows) return MI_ERR_UNSUPPORTED;
     a.Hq = static_cast<int>(Hq);
     a.Hkv = static_cast<int>(Hkv);
     a.G = static_cast<int>(Hq / Hkv);

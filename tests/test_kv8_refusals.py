@@ -244,3 +244,11 @@ def test_the_plain_rounding():
     assert same.sum() > 500
     np.testing.assert_array_equal(R.to_e4m3(x)[same], want.view(torch.uint8).numpy()[same])
     assert [R.exponent(a) for a in (0.0, 448.0, 448.5, 2.0 ** -24, 65504.0, 57344.0)] == [-32, 0, 1, -32, 8, 7]
+
+
+def test_attention_numbers_a_sequences_rows_in_31_bits(lib):
+    """S tokens of Hq / Hkv heads each: 2^21 of 1024 are 2^31 rows."""
+    most = ((1 << 31) - 1 - 128) // 1024
+    for S, ok in ((1 << 24, False), (1 << 21, False), (most + 1, False), (most, True)):
+        n = lib.mi_kv8_attention_workspace_bytes(1024, 1, 16, segs(seg(S=S)), 1)
+        assert (n >= 0) if ok else (n == UNSUPPORTED), (S, n)
