@@ -1086,8 +1086,8 @@ def kv8_scatter(k, v, k_cache, v_cache, k_scale, v_scale, layer: int, segments, 
                                             stream)
     if r is not None:
         return r
-    L, NB, Hkv, bs, hd = _kv8_checks(k_cache, v_cache, k_scale, v_scale, layer, k)
     ks, vs = _need_rows(k, "k"), _need_rows(v, "v")
+    L, NB, Hkv, bs, hd = _kv8_checks(k_cache, v_cache, k_scale, v_scale, layer, k)
     T = k.shape[0]
     if tuple(k.shape) != (T, Hkv, hd) or v.shape != k.shape:
         raise ValueError("k and v must be [T, Hkv, hd] as the cache is")
