@@ -58,17 +58,10 @@ __device__ __forceinline__ void v_pair(const uint32_t (&raw)[Tile<HD>::kKl][Tile
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
         const int k = 8 * m + 2 * p;
-        h2 a, b;
-        if (hi) {
-            a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[k][word], scale, true);
-            b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[k + 1][word], scale, true);
-        } else {
-            a = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[k][word], scale, false);
-            b = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(raw[k + 1][word], scale, false);
-        }
-        const uint32_t ua = __builtin_bit_cast(uint32_t, a), ub = __builtin_bit_cast(uint32_t, b);
-        e[p] = __builtin_amdgcn_perm(ub, ua, 0x05040100u);
-        o[p] = __builtin_amdgcn_perm(ub, ua, 0x07060302u);
+        // two keys' bytes of d and of d + 1, side by side
+        const uint32_t w = __builtin_amdgcn_perm(raw[k + 1][word], raw[k][word], hi ? 0x07030602u : 0x05010400u);
+        e[p] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, false));
+        o[p] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, true));
     }
     typedef uint32_t u4 __attribute__((ext_vector_type(4)));
     even = __builtin_bit_cast(h8, u4{e[0], e[1], e[2], e[3]});

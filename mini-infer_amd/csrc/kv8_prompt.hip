@@ -210,14 +210,10 @@ __global__ __launch_bounds__(256, HD > 128 ? 1 : 2) void kv8_prompt_kernel(Kv8At
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const h2 x = j ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(vraw[2 * i], scale, true)
-                                   : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(vraw[2 * i], scale, false);
-                    const h2 y = j ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(vraw[2 * i + 1], scale, true)
-                                   : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(vraw[2 * i + 1], scale, false);
-                    const uint32_t ux = __builtin_bit_cast(uint32_t, x), uy = __builtin_bit_cast(uint32_t, y);
-                    w[2 * j][i] = __builtin_amdgcn_perm(uy, ux, 0x05040100u);
-                    w[2 * j + 1][i] = __builtin_amdgcn_perm(uy, ux, 0x07060302u);
+                for (int j = 0; j < 2; ++j) {  // two keys' bytes of d and of d + 1, side by side
+                    const uint32_t x = __builtin_amdgcn_perm(vraw[2 * i + 1], vraw[2 * i], j ? 0x07030602u : 0x05010400u);
+                    w[2 * j][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, false));
+                    w[2 * j + 1][i] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(x, scale, true));
                 }
             }
 #pragma unroll
