@@ -25,16 +25,20 @@
 
 namespace mi {
 
-// Which of the two kernels a segment takes.  Tiles of 16 rows read every key once each, tiles of
-// 128 once for all, but need many sequences, heads or rows to fill the GPU.  Measured, tiles of 16
-// against 128 (us), by the number of 16-row tiles: head_dim 128, a prompt's chunk at 8000: 228 tiles 93 / 87,
-// 452 143 / 128; two at 2000: 232 44 / 56, 456 67 / 60; head_dim 64: 544 39 / 44, 1056 68 / 60; head_dim
-// 256, which takes tiles of 128 at a wave per SIMD: 528 63 / 78, 1040 111 / 100.
-constexpr int kFewRows = 64;  // rows of a (sequence, KV head) that always go in tiles of 16
-constexpr int64_t few_tiles(int64_t hd) { return hd <= 64 ? 700 : hd <= 128 ? 400 : 1000; }
+// Which of the two kernels a segment takes.  Tiles of 16 rows read their keys once each, tiles of
+// 128 once for all, but leave CUs idle where there are few.  By the number of 16-row tiles; tiles
+// of 16 against 128 (us), 28 heads on 4 of 128: a chunk at 8000 228 tiles 75 / 84, 452 117 / 124, 900 226 / 138;
+// 16 chunks at 4000 256 tiles 52 / 62, 512 75 / 70; 64 at 500 1024 53 / 23.  16 heads of 64: 544 tiles
+// 38 / 41, 768 67 / 78, 1056 67 / 57.  8 heads on 4 of 256, where a CU holds one workgroup with tiles of 128:
+// 528 tiles 63 / 75, 1040 111 / 97, but 1280 in 64 sequences of 66 rows 101 / 152.
+constexpr int64_t few_rows(int64_t hd) { return hd <= 128 ? 16 : 96; }  // that always go in tiles of 16
+constexpr int64_t few_tiles(int64_t hd) { return hd <= 64 ? 800 : hd <= 128 ? 480 : 1000; }
 std::atomic<int> g_kv8_tile{0};  // mi_kv8_attention_test_tile
 constexpr int kRows = 16;      // query rows of a tile: (token, head of the KV head's group)
-constexpr int64_t kWant = 1024;        // workgroups that a segment of few rows is split into
+// Workgroups that a segment of few rows is split into: two for each CU, which holds one at a time.
+// Uniform lengths would take one (64 sequences of 5000: 66 us with 256, 76 with 512, 83 with 1024),
+// ragged ones need the second (100 to 12000: 105, 90, 107).
+constexpr int64_t kWant = 512;
 constexpr int64_t kPromptWant = 512;   // and one of many rows
 constexpr int64_t kCounters = kKv8Segs * 1024;  // at the head of the workspace, zeros between calls
 
@@ -75,10 +79,10 @@ __device__ __forceinline__ void v_pair(const uint32_t (&raw)[Tile<HD>::kKl][Tile
 // step (8 KB at head_dim 128) in flight while it computes.
 //
 // Bound by HBM where the caches are long: 64 sequences of 100 to 28000 tokens, 28 query heads on 4,
-// head_dim 128, 0.92 GB in 196 us, 4.7 TB/s, 92% of what a large copy reaches; 24 sequences in a
-// window of 1024, head_dim 256, 50 MB in 21 us.  Short ones are bound by the chain from the sequence's
+// head_dim 128, 0.92 GB in 179 us, 5.1 TB/s, what a large copy reaches; 24 sequences in a
+// window of 1024, head_dim 256, 50 MB in 20 us.  Short ones are bound by the chain from the sequence's
 // length to the join: one sequence of 517 tokens 11.3 us (14.4 with four waves to a workgroup).  At
-// least two steps a wave in a split: with one the 64 sequences take 225 us, with four 209.
+// least two steps a wave in a split: with one the window takes 28 us, with four 26.
 template <int HD>
 __global__ __launch_bounds__(Tile<HD>::kWaves * 64, 2) void kv8_attn_kernel(Kv8Attn a) {
     using L = Tile<HD>;
@@ -425,7 +429,7 @@ static int kv8_attn_plan(const Kv8Attn& all, Kv8Attn& few, Kv8Attn& many, int64_
     for (int i = 0; i < all.sg.n; ++i) {
         const int64_t rows = all.sg.S[i] * all.G;
         const int64_t tiles16 = all.sg.B[i] * ceil_div(rows, kRows) * all.Hkv;
-        const bool wide = asked == 0 ? rows > kFewRows && tiles16 >= few_tiles(all.hd) : asked != kRows;
+        const bool wide = asked == 0 ? rows > few_rows(all.hd) && tiles16 >= few_tiles(all.hd) : asked != kRows;
         Kv8Attn& a = wide ? many : few;
         const int n = a.sg.n++;
         a.sg.off[n] = all.sg.off[i];
