@@ -19,6 +19,7 @@
 #include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <type_traits>
 
 #include "kv8_attn.h"
 #include "mi_host.h"
@@ -39,12 +40,17 @@ constexpr int kRows = 16;      // query rows of a tile: (token, head of the KV h
 // Uniform lengths would take one (64 sequences of 5000: 66 us with 256, 76 with 512, 83 with 1024),
 // ragged ones need the second (100 to 12000: 105, 90, 107).
 constexpr int64_t kWant = 512;
+// Tiles of a call from which a workgroup has four waves, two workgroups to a CU: one's loads go on while the
+// other begins and ends.  1024 tiles (128 sequences, 8 KV heads of 128) of 1000 keys 50 us, 62 with eight
+// waves, of 100 to 12000 289 and 298; fewer tiles of ragged lengths want the longest one's keys on eight waves
+// (512 tiles of 100 to 12000: 184 and 150).
+constexpr int64_t kFill = 1024;
 constexpr int64_t kPromptWant = 512;   // and one of many rows
 constexpr int64_t kCounters = kKv8Segs * 1024;  // at the head of the workspace, zeros between calls
 
-template <int HD>
+template <int HD, int WAVES>
 struct Tile {
-    static constexpr int kWaves = 8;             // of a workgroup, each on every eighth step; two a SIMD
+    static constexpr int kWaves = WAVES;         // of a workgroup, each on every WAVES-th step; two a SIMD
     static constexpr int kLeast = 2 * kWaves;    // steps of a split, and what they are a multiple of
     static constexpr int kKl = HD > 128 ? 8 : 16;  // keys of a step that a lane group has
     static constexpr int kKeys = 4 * kKl;            // keys of a wave's step
@@ -55,8 +61,8 @@ struct Tile {
 };
 
 // V's d column `j` of keys 8m .. 8m + 7 of the lane's block, as an MFMA operand.
-template <int HD>
-__device__ __forceinline__ void v_pair(const uint32_t (&raw)[Tile<HD>::kKl][Tile<HD>::kVw], int m, int word, int hi,
+template <int KL, int VW>
+__device__ __forceinline__ void v_pair(const uint32_t (&raw)[KL][VW], int m, int word, int hi,
                                        float scale, h8& even, h8& odd) {
     uint32_t e[4], o[4];
 #pragma unroll
@@ -83,9 +89,9 @@ __device__ __forceinline__ void v_pair(const uint32_t (&raw)[Tile<HD>::kKl][Tile
 // window of 1024, head_dim 256, 50 MB in 20 us.  Short ones are bound by the chain from the sequence's
 // length to the join: one sequence of 517 tokens 11.3 us (14.4 with four waves to a workgroup).  At
 // least two steps a wave in a split: with one the window takes 28 us, with four 26.
-template <int HD>
-__global__ __launch_bounds__(Tile<HD>::kWaves * 64, 2) void kv8_attn_kernel(Kv8Attn a) {
-    using L = Tile<HD>;
+template <int HD, int WAVES>
+__global__ __launch_bounds__(WAVES * 64, 2) void kv8_attn_kernel(Kv8Attn a) {
+    using L = Tile<HD, WAVES>;
     constexpr int kWaves = L::kWaves, kThreads = kWaves * 64, KL = L::kKl, NT = KL / 4, kKeys = L::kKeys;
     __shared__ float s_ml[kWaves][2][kRows];
     __shared__ float s_o[kWaves][kRows][HD + 4];
@@ -269,7 +275,7 @@ __global__ __launch_bounds__(Tile<HD>::kWaves * 64, 2) void kv8_attn_kernel(Kv8A
 #pragma unroll
             for (int k = 0; k < KL / 8; ++k) {
                 h8 even, odd;
-                v_pair<HD>(vr, k, j >> 2, (j >> 1) & 1, vscale, even, odd);
+                v_pair(vr, k, j >> 2, (j >> 1) & 1, vscale, even, odd);
                 o[j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, p[k], o[j], 0, 0, 0);
                 o[j + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, p[k], o[j + 1], 0, 0, 0);
             }
@@ -293,7 +299,7 @@ __global__ __launch_bounds__(Tile<HD>::kWaves * 64, 2) void kv8_attn_kernel(Kv8A
 #pragma unroll
                 for (int k = 0; k < KL / 8; ++k) {
                     h8 even, odd;
-                    v_pair<HD>(vr, k, j >> 2, (j >> 1) & 1, 1.0f, even, odd);
+                    v_pair(vr, k, j >> 2, (j >> 1) & 1, 1.0f, even, odd);
                     n0 = __builtin_amdgcn_mfma_f32_16x16x32_f16(even, see[k], n0, 0, 0, 0);
                     n1 = __builtin_amdgcn_mfma_f32_16x16x32_f16(odd, see[k], n1, 0, 0, 0);
                 }
@@ -564,9 +570,16 @@ extern "C" int mi_kv8_attention_f16(const void* q, int64_t q_stride, const void*
     if (many.sg.n > 0) kv8_prompt_launch(many, s);
     if (few.sg.n > 0) {
         const dim3 grid(static_cast<unsigned>(few.first[few.sg.n]));
-        if (head_dim <= 64) kv8_attn_kernel<64><<<grid, dim3(Tile<64>::kWaves * 64), 0, s>>>(few);
-        else if (head_dim <= 128) kv8_attn_kernel<128><<<grid, dim3(Tile<128>::kWaves * 64), 0, s>>>(few);
-        else kv8_attn_kernel<256><<<grid, dim3(Tile<256>::kWaves * 64), 0, s>>>(few);
+        int64_t groups = 0;
+        for (int i = 0; i < few.sg.n; ++i) groups += few.sg.B[i] * few.tiles[i] * few.Hkv;
+        const auto launch = [&](auto width) {
+            constexpr int HD = decltype(width)::value;
+            if (groups < kFill) kv8_attn_kernel<HD, 8><<<grid, dim3(512), 0, s>>>(few);
+            else kv8_attn_kernel<HD, 4><<<grid, dim3(256), 0, s>>>(few);
+        };
+        if (head_dim <= 64) launch(std::integral_constant<int, 64>{});
+        else if (head_dim <= 128) launch(std::integral_constant<int, 128>{});
+        else launch(std::integral_constant<int, 256>{});
     }
     return launch_status();
 }

@@ -130,6 +130,16 @@ def test_either_side_of_the_choice(mk, dev, Hq, Hkv, hd, S, B):
     assert mk.kv8_attention_workspace_bytes(Hq, Hkv, hd, R.dev_segments(c.segs, dev)) == n
 
 
+@pytest.mark.parametrize("Hq,Hkv,hd", [(16, 8, 64), (24, 8, 128), (16, 16, 80), (8, 8, 256)])
+def test_many_sequences(mk, dev, Hq, Hkv, hd):
+    """More tiles than the GPU holds workgroups, beside a few of a long sequence."""
+    rng = np.random.default_rng(hd)
+    lens = rng.integers(0, 300, 130).tolist() + [1, 64, 65]
+    c = Case(hd, Hq, Hkv, hd, 16, [(1, [(max(n - 1, 0), n) for n in lens]), (2, [(1998, 2000)])]).unused()
+    c.check(mk, dev)
+    c.check(mk, dev, window=70)
+
+
 @pytest.mark.parametrize("hd", [64, 128, 256])
 def test_long_sequences_in_splits(mk, dev, hd):
     c = Case(hd, 4, 2, hd, 16, [(1, [(4999, 5000), (2300, 2301), (70, 71)])]).unused()
