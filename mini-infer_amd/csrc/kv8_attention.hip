@@ -30,10 +30,9 @@ namespace mi {
 // 128 once for all, but leave CUs idle where there are few.  By the number of 16-row tiles; tiles
 // of 16 against 128 (us), 28 heads on 4 of 128: a chunk at 8000 228 tiles 75 / 84, 452 117 / 124, 900 226 / 138;
 // 16 chunks at 4000 256 tiles 52 / 62, 512 75 / 70; 64 at 500 1024 53 / 23.  16 heads of 64: 544 tiles
-// 38 / 41, 768 67 / 78, 1056 67 / 57.  8 heads on 4 of 256, where a CU holds one workgroup with tiles of 128:
-// 528 tiles 63 / 75, 1040 111 / 97, but 1280 in 64 sequences of 66 rows 101 / 152.
-constexpr int64_t few_rows(int64_t hd) { return hd <= 128 ? 16 : 96; }  // that always go in tiles of 16
-constexpr int64_t few_tiles(int64_t hd) { return hd <= 64 ? 800 : hd <= 128 ? 480 : 1000; }
+// 38 / 41, 768 67 / 78, 1056 67 / 57.  16 heads on 8 of 256: 528 tiles 112 / 121, 640 203 / 184, 1056 81 / 62.
+constexpr int kFewRows = 32;  // that always go in tiles of 16 (64 sequences of 18 rows, 8 of 256: 58 / 77)
+constexpr int64_t few_tiles(int64_t hd) { return hd <= 64 ? 800 : hd <= 128 ? 480 : 600; }
 std::atomic<int> g_kv8_tile{0};  // mi_kv8_attention_test_tile
 constexpr int kRows = 16;      // query rows of a tile: (token, head of the KV head's group)
 // Workgroups that a segment of few rows is split into: two for each CU, which holds one at a time.
@@ -45,7 +44,9 @@ constexpr int64_t kWant = 512;
 // waves, of 100 to 12000 289 and 298; fewer tiles of ragged lengths want the longest one's keys on eight waves
 // (512 tiles of 100 to 12000: 184 and 150).
 constexpr int64_t kFill = 1024;
-constexpr int64_t kPromptWant = 512;   // and one of many rows
+// And one of many rows: what the CUs hold at once, 3, 2 and 1 each.  A chunk of 1024 at 12000, 16 heads of 64: 137
+// us with 512, 115 with 768; 32 on 8 of 128: 274 with 512, 313 with 768; 16 on 8 of 256: 440 with 256, 506 with 512.
+constexpr int64_t prompt_want(int64_t hd) { return hd <= 64 ? 768 : hd <= 128 ? 512 : 256; }
 constexpr int64_t kCounters = kKv8Segs * 1024;  // at the head of the workspace, zeros between calls
 
 template <int HD, int WAVES>
@@ -435,7 +436,7 @@ static int kv8_attn_plan(const Kv8Attn& all, Kv8Attn& few, Kv8Attn& many, int64_
     for (int i = 0; i < all.sg.n; ++i) {
         const int64_t rows = all.sg.S[i] * all.G;
         const int64_t tiles16 = all.sg.B[i] * ceil_div(rows, kRows) * all.Hkv;
-        const bool wide = asked == 0 ? rows > few_rows(all.hd) && tiles16 >= few_tiles(all.hd) : asked != kRows;
+        const bool wide = asked == 0 ? rows > kFewRows && tiles16 >= few_tiles(all.hd) : asked != kRows;
         Kv8Attn& a = wide ? many : few;
         const int n = a.sg.n++;
         a.sg.off[n] = all.sg.off[i];
@@ -447,7 +448,7 @@ static int kv8_attn_plan(const Kv8Attn& all, Kv8Attn& few, Kv8Attn& many, int64_
         a.sg.sp[n] = all.sg.sp[i];
         const int64_t tile = wide ? kPromptRows : kRows, tiles = ceil_div(rows, tile);
         const int64_t groups = a.sg.B[n] * tiles * a.Hkv;
-        const int64_t ns = std::clamp<int64_t>((wide ? kPromptWant : kWant) / std::max<int64_t>(groups, 1), 1,
+        const int64_t ns = std::clamp<int64_t>((wide ? prompt_want(all.hd) : kWant) / std::max<int64_t>(groups, 1), 1,
                                                std::min<int64_t>(a.sg.mb[n], wide ? kPromptSplits : kMaxSplits));
         a.tiles[n] = static_cast<int>(tiles);
         a.nsplit[n] = static_cast<int>(ns);
